@@ -221,6 +221,19 @@ int sglamd_int8_scaled_mm(const void* a, int64_t lda, const void* b, int64_t ldb
                           const void* bias, void* out, int64_t ldc, int out_dtype, int64_t M, int64_t N, int64_t K,
                           void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The same product of activation rows with a zero point each (asymmetric codes):
+ *   out = cast( float(acc_i32 - zp[m] * weight_sums[n]) * (sb[n] * sa[m]) + float(bias[n]) ),
+ * i.e. sum_k (a[m, k] - zp[m]) * b[n, k], exact as long as it fits 32 bits, which it does for zero points in [-128, 127]
+ * and K <= 65536 (longer K: SGLAMD_ENOTSUP).  zp int32[M], |zp| < 2^23; weight_sums int32[N], the sums of the weight rows
+ * (sglamd_int8_weight_sums), kept with the weight.  The reference has the symmetric product only. */
+int sglamd_int8_scaled_mm_azp(const void* a, int64_t lda, const void* b, int64_t ldb, const float* sa, const float* sb,
+                              const int32_t* zp, const int32_t* weight_sums, const void* bias, void* out, int64_t ldc,
+                              int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                              void* stream);
+
+/* sums[n] = sum over k of b[n, k], b int8 [N, K] with rows of ldb bytes, any K below 2^24 and any alignment. */
+int sglamd_int8_weight_sums(const void* b, int64_t ldb, int64_t N, int64_t K, int32_t* sums, void* stream);
+
 /* Optional scratch for the three GEMM entry points above.  For shapes whose tile grid alone cannot fill the
  * chip (few rows or few columns with a long K) the kernels split K and sum fp32 partial tiles from
  * `workspace`; this returns the number of bytes with which that pays for (M, N, K), or 0.  The GEMMs accept
@@ -427,6 +440,55 @@ int sglamd_fused_rms_fp8_group_quant(const void* x1, int64_t x1_row_stride, cons
                                      void* y1_unquantized, void* res_out, const void* x2, int64_t x2_row_stride,
                                      const void* w2, float eps2, int64_t N2, void* y2, int dtype, int weight_dtype,
                                      int group_size, void* stream);
+
+/* Rows in 8 bits with one scale per row, fused with what produces them.  Nothing is rounded between the inputs and the
+ * codes; with y the row before its codes:
+ *   FP8_E4M3:  scale = max|y| / 448, or *fixed_scale where given;  code = e4m3(clamp(y * (1 / scale), +-448)), zeros for
+ *              a scale of zero
+ *   I8:        amax = max(max|y|, 1e-10), scale = amax / 127;  code = round_half_away(y * (127 / amax))
+ *   I8 with output_zp:  lo = min(0, min y), hi = max(0, max y), scale = max(hi - lo, 1e-10) / 255,
+ *              zp = rint(-128 - lo / scale);  code = clamp(rint(y * (1 / scale)) + zp, -128, 127);  y is scale * (code - zp)
+ * output_q [rows, hidden], output_s fp32 [rows] (a fixed scale is repeated), output_zp int32 [rows] or NULL.  Rows may have
+ * any length, stride (in elements, 0 included) and alignment; lengths that are multiples of 8, at most 32768, in 16-byte
+ * aligned rows are read once in 16-byte pieces, all others value by value, twice.  Outputs overlap no input.  A row that
+ * holds a NaN or an infinity gets a scale that is NaN or infinite (a fixed scale: NaN codes), so that it stays visible
+ * behind the product.
+ *
+ * sglamd_fused_rms_row_quant: v = f32(x) + f32(res), res_out = cast(v), y = v * weight * (1 / sqrt(mean(v^2) + eps)), the
+ *   optional output y = cast(y).  x, res, y, res_out in dtype (F16/BF16), y and res_out [rows, hidden] contiguous; weight
+ *   [hidden] of F32 or dtype; res and res_out go together (NULL: none).  A sum of squares beyond fp32 counts as infinite.
+ *   Stands beside sglamd_fused_rms_fp8_group_quant for the row-scaled products (sglamd_fp8_scaled_mm, sglamd_int8_scaled_mm).
+ * sglamd_silu_mul_row_quant: y = gate / (1 + exp(-gate)) * up, x rows of [gate | up], 2 * hidden values, F16/BF16.
+ * sglamd_per_token_quant_int8_asym: y = x, with zero points; F32/F16/BF16. */
+int sglamd_fused_rms_row_quant(const void* x, int64_t x_row_stride, const void* res, int64_t res_row_stride,
+                               const void* weight, float eps, const float* fixed_scale, int64_t rows, int64_t hidden,
+                               void* output_q, float* output_s, int32_t* output_zp, void* y, void* res_out, int dtype,
+                               int weight_dtype, int q_dtype, void* stream);
+int sglamd_silu_mul_row_quant(const void* x, int64_t x_row_stride, const float* fixed_scale, int64_t rows,
+                              int64_t hidden, void* output_q, float* output_s, int32_t* output_zp, int dtype,
+                              int q_dtype, void* stream);
+int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_stride, int dtype, int64_t rows, int64_t hidden,
+                                     int8_t* output_q, float* output_s, int32_t* output_zp, void* stream);
+
+/* The gated-SiLU expert layer of a few tokens whose rows are in 8 bits already (the codes and scales that
+ * sglamd_fused_rms_row_quant or the per-token quantisers write), experts with a scale per output channel, in two launches:
+ *   h = x_scale[t] * w13_scale[e] * (x[t] . w13[e]) (+ b13[e]);  a = silu(gate) * up in fp32, in 8 bits per (token, expert)
+ *   pair by the symmetric formulas above;  out[t] = cast( routed_scaling_factor * sum over the token's pairs, in their order, of
+ *   topk_weights * (a_scale * w2_scale[e] * (a . w2[e]) (+ b2[e])) ).
+ * Against sglamd_fused_moe_layer it takes quantised rows and rounds nothing to 16 bits on the way.  Bits depend on neither
+ * the order of arrivals nor the launch.
+ * x [M, H] e4m3fn or int8 (q_dtype), contiguous; w13 [E, 2 * I, H] (gate rows, then up rows), w2 [E, H, I] of that type;
+ * w13_scale fp32 [E, 2 * I], w2_scale [E, H]; b13, b2 optional, shaped like the scales, in out_dtype (F16/BF16);
+ * topk_weights fp32 [M, topk], topk_ids [M, topk] int32 or int64: pairs whose id is outside [0, E) contribute nothing, an
+ * id may be named more than once.  H and I multiples of 16, I <= 16384, M * topk <= 64 (more: SGLAMD_ENOTSUP).  workspace:
+ * sglamd_fused_experts_few_tokens_workspace(...) bytes, 16-byte aligned, nothing in it has to start at zero; calls that
+ * overlap need workspaces of their own. */
+int64_t sglamd_fused_experts_few_tokens_workspace(int64_t M, int64_t I, int topk);
+int sglamd_fused_experts_few_tokens(const void* x, const float* x_scale, int q_dtype, int64_t M, int64_t H, int64_t I,
+                                    int E, int topk, const void* w13, const float* w13_scale, const void* b13,
+                                    const void* w2, const float* w2_scale, const void* b2, const float* topk_weights,
+                                    const void* topk_ids, int ids_dtype, void* out, int out_dtype,
+                                    float routed_scaling_factor, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The whole block-FP8 MoE layer from one host call (five launches on `stream`):
  *   quantise hidden (1x128 groups) + moe_align_block_size -> grouped GEMM with w13 -> silu*mul + quantise

@@ -36,6 +36,8 @@ SIGNATURES = {
                                        _i64, _p, _i64, _p],
     "sglamd_fp8_scaled_mm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
     "sglamd_int8_scaled_mm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
+    "sglamd_int8_scaled_mm_azp": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
+    "sglamd_int8_weight_sums": [_p, _i64, _i64, _i64, _p, _p],
     "sglamd_gemm_workspace_bytes": [_i64, _i64, _i64],
     "sglamd_last_gemm_kernel": [],
     "sglamd_last_streaming_shape": [],
@@ -70,6 +72,11 @@ SIGNATURES = {
                                                 _p],
     "sglamd_fused_rms_fp8_group_quant": [_p, _i64, _p, _f, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _f, _i64, _p,
                                          _i, _i, _i, _p],
+    "sglamd_fused_rms_row_quant": [_p, _i64, _p, _i64, _p, _f, _p, _i64, _i64, _p, _p, _p, _p, _p, _i, _i, _i, _p],
+    "sglamd_silu_mul_row_quant": [_p, _i64, _p, _i64, _i64, _p, _p, _p, _i, _i, _p],
+    "sglamd_per_token_quant_int8_asym": [_p, _i64, _i, _i64, _i64, _p, _p, _p, _p],
+    "sglamd_fused_experts_few_tokens_workspace": [_i64, _i64, _i],
+    "sglamd_fused_experts_few_tokens": [_p, _p, _i, _i64, _i64, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _f, _p, _i64, _p],
     "sglamd_prepare_moe_input": [_p, _i64, _i, _i, _i64, _i64, _p, _p, _p, _p, _p, _p, _p],
     "sglamd_shuffle_rows": [_p, _p, _p, _i64, _i64, _p],
     "sglamd_apply_shuffle_mul_sum": [_p, _p, _p, _p, _i, _i64, _i, _i64, _p],

@@ -15,6 +15,7 @@ extern template int dispatch_quantising<GEMM_BLOCK_FP8, true>(const GemmArgs&, i
 extern template int dispatch_quantising<GEMM_ROW_FP8, false>(const GemmArgs&, int, hipStream_t, bool);
 extern template int dispatch_out<GEMM_ROW_FP8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 extern template int dispatch_out<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
+extern template int dispatch_out_zero_point<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 extern template int dispatch_out<GEMM_BLOCK_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 
 static int check_common(const char* op, const void* a, const void* b, const void* c, int64_t M, int64_t N, int64_t K,
@@ -173,7 +174,8 @@ extern "C" int sglamd_int8_blockwise_scaled_mm(const void* a, int64_t lda, const
 
 static int rowwise(int mode, const char* op, const void* a, int64_t lda, const void* b, int64_t ldb, const float* sa,
                    const float* sb, const void* bias, void* out, int64_t ldc, int out_dtype, int64_t M, int64_t N,
-                   int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {
+                   int64_t K, void* workspace, int64_t workspace_bytes, void* stream, const int32_t* zp = nullptr,
+                   const int32_t* weight_sums = nullptr) {
   const DeviceScope scope;
   int rc = check_common(op, a, b, out, M, N, K, lda, ldb, ldc);
   if (rc) return rc;
@@ -186,6 +188,8 @@ static int rowwise(int mode, const char* op, const void* a, int64_t lda, const v
   g.ldb = ldb;
   g.sa = sa;
   g.sb = sb;
+  g.A16 = zp;
+  g.route_ids = weight_sums;
   g.bias = bias;
   g.C = out;
   g.ldc = ldc;
@@ -193,6 +197,7 @@ static int rowwise(int mode, const char* op, const void* a, int64_t lda, const v
   g.N = (int)N;
   g.K = (int)K;
   if (mode == GEMM_ROW_FP8) return dispatch_out<GEMM_ROW_FP8>(g, out_dtype, (hipStream_t)stream, workspace, workspace_bytes);
+  if (zp) return dispatch_out_zero_point<GEMM_ROW_INT8>(g, out_dtype, (hipStream_t)stream, workspace, workspace_bytes);
   return dispatch_out<GEMM_ROW_INT8>(g, out_dtype, (hipStream_t)stream, workspace, workspace_bytes);
 }
 
@@ -244,6 +249,18 @@ extern "C" int sglamd_int8_scaled_mm(const void* a, int64_t lda, const void* b, 
                                      void* stream) {
   return rowwise(GEMM_ROW_INT8, "int8_scaled_mm", a, lda, b, ldb, sa, sb, bias, out, ldc, out_dtype, M, N, K, workspace,
                  workspace_bytes, stream);
+}
+
+extern "C" int sglamd_int8_scaled_mm_azp(const void* a, int64_t lda, const void* b, int64_t ldb, const float* sa, const float* sb,
+                                         const int32_t* zp, const int32_t* weight_sums, const void* bias, void* out, int64_t ldc,
+                                         int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                                         void* stream) {
+  const char* op = "int8_scaled_mm_azp";
+  SGLAMD_REQUIRE(zp && weight_sums, SGLAMD_EINVAL, "%s: null zero points or weight sums", op);
+  // (sums of 65536 products of a code less its zero point, 255 at most, and a weight stay inside 32 bits)
+  SGLAMD_REQUIRE(K <= 65536, SGLAMD_ENOTSUP, "%s: K (%lld) is beyond 65536", op, (long long)K);
+  return rowwise(GEMM_ROW_INT8, op, a, lda, b, ldb, sa, sb, bias, out, ldc, out_dtype, M, N, K, workspace, workspace_bytes, stream, zp,
+                 weight_sums);
 }
 
 extern "C" int sglamd_last_gemm_kernel(void) { return last_kernel; }

@@ -572,6 +572,7 @@ __global__ __launch_bounds__(128 * WGN) void gemm8_big_kernel(GemmArgs g) {
   __syncthreads();
   // row modes: the weight-row scales (and bias) of this lane's 32 columns, fetched once for all row tiles
   float sbn[2][4][4], bia[2][4][4];
+  int sums[out_zero_point<OT> ? 2 : 1][4][4];
   if constexpr (!gemm_is_block(MODE)) {
     const float* sb_row = g.sb + (MOE ? (int64_t)max(expert, 0) * g.sb_se : 0);
     const OS* bias = g.bias ? (const OS*)g.bias + (MOE ? (int64_t)max(expert, 0) * g.sb_sk : 0) : nullptr;
@@ -584,6 +585,7 @@ __global__ __launch_bounds__(128 * WGN) void gemm8_big_kernel(GemmArgs g) {
           const int nn = min(n0 + wn * 64 + j * 32 + 8 * rq + 4 * fk + r, (int)g.N - 1);
           sbn[j][rq][r] = sb_row[MOE ? (int64_t)nn * g.sb_sn : nn];
           bia[j][rq][r] = bias ? OT::to_f32(bias[nn]) : 0.f;
+          if constexpr (out_zero_point<OT>) sums[j][rq][r] = ((const int32_t*)g.route_ids)[nn];
         }
   }
 #pragma unroll
@@ -601,6 +603,8 @@ __global__ __launch_bounds__(128 * WGN) void gemm8_big_kernel(GemmArgs g) {
     }
     float sam = 1.f;
     if (!gemm_is_block(MODE)) sam = g.sa[MOE ? (int64_t)(m / g.top_k) * g.sa_sm : m];
+    int minus_zp = 0;
+    if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[m];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
 #pragma unroll
@@ -608,7 +612,10 @@ __global__ __launch_bounds__(128 * WGN) void gemm8_big_kernel(GemmArgs g) {
         const int cl = wn * 64 + j * 32 + 8 * rq + 4 * fk;
         float v[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = (float)acc[i][j][rq * 4 + r];
+        for (int r = 0; r < 4; r++) {
+          if constexpr (out_zero_point<OT>) v[r] = (float)zero_point_off((int)acc[i][j][rq * 4 + r], minus_zp, sums[j][rq][r]);
+          else v[r] = (float)acc[i][j][rq * 4 + r];
+        }
         if constexpr (!gemm_is_block(MODE)) {
 #pragma unroll
           for (int r = 0; r < 4; r++) {
@@ -689,6 +696,21 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float* __restr
     if constexpr (MODE == GEMM_ROW_INT8) {
       v4i a = *(const v4i*)(ws + e);
       for (int s = 1; s < slices; s++) a += *(const v4i*)(ws + (int64_t)s * g.M * g.N + e);
+      if constexpr (out_zero_point<OT>) {
+        const int minus_zp = -((const int32_t*)g.A16)[e / g.N];
+        const int32_t* sums = (const int32_t*)g.route_ids + e % g.N;
+        int w[4];
+        if ((((uintptr_t)g.route_ids) & 15) == 0) {
+          const v4i s4 = *(const v4i*)sums;
+#pragma unroll
+          for (int r = 0; r < 4; r++) w[r] = s4[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++) w[r] = sums[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) a[r] = zero_point_off(a[r], minus_zp, w[r]);
+      }
 #pragma unroll
       for (int r = 0; r < 4; r++) v[r] = (float)a[r];
     } else {

@@ -49,6 +49,20 @@ __device__ __forceinline__ v4i add_bias8(v4i v, v4i b) {
   return v;
 }
 
+// Output type of a dense INT8 product whose activation rows have a zero point each: sum_k (a - zp) w = sum_k a w - zp * sum_k w,
+// with zp[m] behind GemmArgs::A16 and the weight rows' sums behind GemmArgs::route_ids, int32 both (two words that the dense
+// kernels do not use otherwise).  A type for the same reason.  In 32 bits that wrap, as the accumulators do: only the
+// difference has to fit.  The factors of the product are below 2^23, which one full-rate instruction multiplies.
+template <typename T>
+struct ZeroPoint : T {};
+template <typename T>
+constexpr bool out_zero_point = false;
+template <typename T>
+constexpr bool out_zero_point<ZeroPoint<T>> = true;
+__device__ __forceinline__ int zero_point_off(int acc, int minus_zp, int weight_sum) {
+  return (int)((uint32_t)acc + (uint32_t)__mul24(minus_zp, weight_sum));
+}
+
 struct GemmArgs {
   const uint8_t* A;
   int64_t lda;
@@ -78,7 +92,7 @@ struct GemmArgs {
   // skinny MoE kernel with in-kernel activation quantisation: the 16-bit rows that take A's place.
   // (The persistent MoE kernel with the activation in its epilogue has no such rows and finds the address of
   // the group scales it writes, fp32 [pairs, N / 256] at lda16 floats from row to row, here: one more argument word would
-  // cost a scalar register.)
+  // cost a scalar register.)  ZeroPoint output types: the activation rows' zero points.
   const void* A16;
   int64_t lda16;       // bytes between rows
   int act_mode;        // 1: quantise the rows of A16 in the kernel
@@ -92,7 +106,7 @@ struct GemmArgs {
   float sum_scale;
   int* sum_count;
   int sum_tiles;
-  // skinny MoE kernel of one token: topk_ids as handed to the layer
+  // skinny MoE kernel of one token: topk_ids as handed to the layer.  (ZeroPoint output types: the weight rows' sums.)
   const void* route_ids;
   int route_ids_i64;
   int route_experts;
@@ -393,6 +407,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(GA ga) {
     if (!row_ok) continue;
     float sam = 1.f;
     if (!gemm_is_block(MODE)) sam = MOE ? g.sa[(out_row / g.top_k) * gx.row_sa_stride] : g.sa[out_row];
+    int minus_zp = 0;
+    if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[out_row];
     OS* crow = (OS*)g.C + out_row * g.ldc;
     const OS* bias = g.bias ? (const OS*)g.bias + (MOE ? (int64_t)max(expert, 0) * gx.bias_se : 0) : nullptr;
 #pragma unroll
@@ -410,6 +426,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(GA ga) {
           const float sbn = (n + r) < g.N ? (MOE ? sb_base[(int64_t)(n + r) * gx.row_sb_stride] : g.sb[n + r]) : 0.f;
           if constexpr (MODE == GEMM_ROW_FP8) {
             v[r] = acc[i][j][r] * sbn * sam;
+          } else if constexpr (out_zero_point<OT>) {
+            v[r] = (float)zero_point_off(acc[i][j][r], minus_zp, (n + r) < g.N ? ((const int32_t*)g.route_ids)[n + r] : 0) * (sbn * sam);
           } else {
             v[r] = (float)acc[i][j][r] * (sbn * sam);
           }

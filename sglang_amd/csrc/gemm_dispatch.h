@@ -196,7 +196,7 @@ static int dispatch_dense(const GemmArgs& g, hipStream_t st, void* workspace, in
   strip_last_shape = skinny_last_shape = 0;
   if (big && may_split && g.M > 16) {
     const DenseChoice choice = dense_choice(g.M, g.N, g.K);
-    const StripPlan& plan = choice.strip;
+    const StripPlan plan = strip_plan_for<OT>(choice.strip, g.M);
     if (choice.row_tile && gemm8_skinny_ok(g, g.M)) {
       if (choice.row_tile == 64) return gemm8_skinny_launch<4, MODE, OT, false>(g, st, ceil_div(g.M, 64));
       if (choice.row_tile == 16) return gemm8_skinny_launch<1, MODE, OT, false>(g, st, ceil_div(g.M, 16));
@@ -221,6 +221,7 @@ static int dispatch_dense(const GemmArgs& g, hipStream_t st, void* workspace, in
       rest.C = (OS*)g.C + n1;
       rest.sb = gemm_is_block(MODE) ? g.sb + (n1 >> 7) * g.sb_sn : g.sb + n1;
       if (g.bias) rest.bias = (const OS*)g.bias + n1;
+      if constexpr (out_zero_point<OT>) rest.route_ids = (const int32_t*)g.route_ids + n1;
       int rc = dispatch_dense<MODE, OT>(head, st, workspace, workspace_bytes, false);
       if (rc) return rc;
       const int ran = last_kernel;
@@ -295,6 +296,14 @@ template <int MODE>
 int dispatch_out_biased(const GemmArgs& g, int out_dtype, hipStream_t st, void* ws, int64_t ws_bytes) {
   if (out_dtype == SGLAMD_BF16) return dispatch_dense<MODE, Biased<BF16>>(g, st, ws, ws_bytes);
   if (out_dtype == SGLAMD_F16) return dispatch_dense<MODE, Biased<F16>>(g, st, ws, ws_bytes);
+  return fail(SGLAMD_EINVAL, "out_dtype must be Half or BFloat16");
+}
+
+// The same for activation rows with zero points (gemm_mode_row_int8_zp.hip).
+template <int MODE>
+int dispatch_out_zero_point(const GemmArgs& g, int out_dtype, hipStream_t st, void* ws, int64_t ws_bytes) {
+  if (out_dtype == SGLAMD_BF16) return dispatch_dense<MODE, ZeroPoint<BF16>>(g, st, ws, ws_bytes);
+  if (out_dtype == SGLAMD_F16) return dispatch_dense<MODE, ZeroPoint<F16>>(g, st, ws, ws_bytes);
   return fail(SGLAMD_EINVAL, "out_dtype must be Half or BFloat16");
 }
 

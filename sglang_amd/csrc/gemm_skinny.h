@@ -756,6 +756,8 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
       float sam = 1.f;
       const float* sb_row = g.sb;
       const OS* bias = (const OS*)g.bias;
+      int minus_zp = 0;
+      if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[out_row];
       if constexpr (!gemm_is_block(MODE)) {
         if constexpr (DQ) sam = xq_scales[out_row];
         else sam = g.sa[MOE ? (out_row / g.top_k) * g.sa_sm : out_row];
@@ -773,6 +775,8 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
           const float sbn = (n + r) < g.N ? sb_row[MOE ? (int64_t)(n + r) * g.sb_sn : n + r] : 0.f;
           if constexpr (MODE == GEMM_ROW_FP8) {
             v[r] = a[r] * sbn * sam;
+          } else if constexpr (out_zero_point<OT>) {
+            v[r] = (float)zero_point_off(a[r], minus_zp, (n + r) < g.N ? ((const int32_t*)g.route_ids)[n + r] : 0) * (sbn * sam);
           } else {
             v[r] = (float)a[r] * (sbn * sam);
           }

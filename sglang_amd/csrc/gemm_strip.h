@@ -412,10 +412,22 @@ __global__ __launch_bounds__(512) void gemm8_strip_kernel(GemmArgs g) {
       for (int i = 0; i < RT; i++) {
         float sam = 1.f;
         if constexpr (!BLK) sam = g.sa[min(i * 32 + frow, (int)g.M - 1)];
+        int minus_zp = 0;
+        if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[min(i * 32 + frow, (int)g.M - 1)];
+        v4i sums[out_zero_point<OT> ? 4 : 1];
+        if constexpr (out_zero_point<OT>) {
+          // (four row tiles leave no registers for the columns' sums, which are fetched for each, nor for their addresses: by
+          // buffer loads one serves all columns, and those past N read as zeros)
+          __builtin_amdgcn_sched_barrier(0);
+          const auto sums_rs = __builtin_amdgcn_make_buffer_rsrc((void*)g.route_ids, 0, g.N * 4, 0x00020000);
+#pragma unroll
+          for (int rq = 0; rq < 4; rq++) sums[rq] = __builtin_amdgcn_raw_buffer_load_b128(sums_rs, (nw + 4 * fk) * 4 + rq * 32, 0, 0);
+        }
         float v[16];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           v[r] = (float)acc[i][r];
+          if constexpr (out_zero_point<OT>) v[r] = (float)zero_point_off((int)acc[i][r], minus_zp, sums[r >> 2][r & 3]);
           if constexpr (!BLK) {
             if constexpr (MODE == GEMM_ROW_FP8) v[r] = v[r] * sbn[r] * sam;
             else v[r] = v[r] * (sbn[r] * sam);
@@ -465,6 +477,17 @@ struct StripPlan {
 };
 // Strips of 32 weight rows, and stages in LDS, of the kernel that runs tiles of `rows` weight rows.
 static inline int strip_strips(int64_t M, int rows) { return rows <= 96 && M <= 32 ? 3 : rows <= 128 ? 4 : 5; }
+// Rows with zero points: five strips of four row tiles would spill, so there a tile has at most 128 weight rows.
+template <typename OT>
+constexpr int strip_strips_most(int strips) {
+  return out_zero_point<OT> && strips > 4 ? 4 : strips;
+}
+template <typename OT>
+static inline StripPlan strip_plan_for(const StripPlan& plan, int64_t M) {
+  StripPlan p = plan;
+  if (M > 96 && p.rows > strip_strips_most<OT>(5) * 32) p.rows = strip_strips_most<OT>(5) * 32;
+  return p;
+}
 static inline int strip_depth(int64_t M, int rows) {
   const int ns = strip_strips(M, rows);
   return M > 32 ? strip_stages<2, 4>() : ns == 3 ? strip_stages<1, 3>() : ns == 4 ? strip_stages<1, 4>() : strip_stages<1, 5>();
@@ -540,7 +563,7 @@ static int gemm8_strip_launch(const GemmArgs& whole, const StripPlan& plan, hipS
     constexpr int NS = decltype(ns)::value;
     if (g.M <= 32) return gemm8_strip_start<MODE, OT, 1, NS>(g, st);
     if constexpr (NS == 3) return gemm8_strip_start<MODE, OT, 2, 4>(g, st);
-    else return g.M <= 64 ? gemm8_strip_start<MODE, OT, 2, NS>(g, st) : g.M <= 96 ? gemm8_strip_start<MODE, OT, 3, NS>(g, st) : gemm8_strip_start<MODE, OT, 4, NS>(g, st);
+    else return g.M <= 64 ? gemm8_strip_start<MODE, OT, 2, NS>(g, st) : g.M <= 96 ? gemm8_strip_start<MODE, OT, 3, NS>(g, st) : gemm8_strip_start<MODE, OT, 4, strip_strips_most<OT>(NS)>(g, st);
   };
   const int ns = strip_strips(g.M, plan.rows);
   if (ns == 3) rc = start(std::integral_constant<int, 3>{});

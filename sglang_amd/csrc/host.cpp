@@ -390,6 +390,118 @@ std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>, optional<Tensor>>
 }
 
 // ---------------------------------------------------------------------------------------
+// rows in 8 bits with one scale each (quantization/fused_row_quant.py, int8_kernel.py and int8_utils.py state the contracts)
+// ---------------------------------------------------------------------------------------
+// These functions are all there is of their operators: what has to see an operator (autograd, a tracer, a transform, a tensor
+// subclass) is refused instead of being handed results without their history.
+bool on_device(const Tensor& t) { return t.is_cuda(); }
+bool on_device(const optional<Tensor>& t) { return !t || t->is_cuda(); }
+template <typename... Tensors>
+void refuse_observed(const char* op, const Tensors&... tensors) {
+  TORCH_CHECK((on_device(tensors) && ...), op, ": every tensor must be a CUDA tensor");
+  if (any_observed(tensors...))
+    C10_THROW_ERROR(NotImplementedError, std::string(op) + " has no gradient and takes plain tensors only, outside of tracers and "
+                                                           "transforms (call it under torch.no_grad())");
+}
+
+// The stride between the rows of a 2D tensor with contiguous rows (one row may report any).
+int64_t row_stride(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.dim() == 2, name, " must be 2D");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " rows must be contiguous");
+  return t.size(0) > 1 ? t.stride(0) : t.size(1);
+}
+void check_same_device(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK(t.device() == x.device(), name, " must be on the device of the input");
+}
+
+// Codes, scales and zero points of `rows` rows.
+struct RowCodes {
+  Tensor q, s;
+  optional<Tensor> zp;
+  const float* fixed = nullptr;
+  RowCodes(const Tensor& x, int64_t rows, int64_t hidden, ScalarType q_dtype, bool symmetric, const optional<Tensor>& scale) {
+    TORCH_CHECK(q_dtype == kFp8 || q_dtype == at::kChar, "dtype_quant must be Float8_e4m3fn or Char");
+    TORCH_CHECK(symmetric || q_dtype == at::kChar, "zero points go with Char codes");
+    TORCH_CHECK(hidden > 0, "rows must not be empty");
+    if (scale) {
+      TORCH_CHECK(q_dtype == kFp8, "a given scale goes with Float8_e4m3fn codes");
+      TORCH_CHECK(scale->scalar_type() == at::kFloat && scale->numel() == 1, "scale must be one Float32");
+      check_same_device(*scale, x, "scale");
+      fixed = scale->data_ptr<float>();
+    }
+    q = empty({rows, hidden}, q_dtype, x);
+    s = empty({rows, 1}, at::kFloat, x);
+    if (!symmetric) zp = empty({rows, 1}, at::kInt, x);
+  }
+  int32_t* zero_points() const { return zp ? zp->data_ptr<int32_t>() : nullptr; }
+};
+
+std::tuple<Tensor, Tensor, optional<Tensor>, optional<Tensor>, optional<Tensor>> fused_rms_row_quant(
+    const Tensor& x, const Tensor& w, double eps, const optional<Tensor>& res, ScalarType q_dtype, bool symmetric,
+    const optional<Tensor>& scale, bool want_y) {
+  refuse_observed("fused_rms_row_quant", x, w, res, scale);
+  const int64_t stride = row_stride(x, "inp"), rows = x.size(0), hidden = x.size(1);
+  const ScalarType t = x.scalar_type();
+  TORCH_CHECK(is_half(t), "inp must be Half or BFloat16");
+  TORCH_CHECK(w.dim() == 1 && w.numel() == hidden && w.is_contiguous(), "weight must be contiguous [hidden]");
+  TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == t, "weight must be Float32 or of the input's dtype");
+  check_same_device(w, x, "weight");
+  int64_t res_stride = 0;
+  if (res) {
+    TORCH_CHECK(res->sizes() == x.sizes() && res->scalar_type() == t, "res must match inp");
+    check_same_device(*res, x, "res");
+    res_stride = row_stride(*res, "res");
+  }
+  const c10::DeviceGuard guard(x.device());
+  const RowCodes o(x, rows, hidden, q_dtype, symmetric, scale);
+  optional<Tensor> y, res_out;
+  if (want_y) y = empty({rows, hidden}, t, x);
+  if (res) res_out = empty({rows, hidden}, t, x);
+  if (rows)
+    check(sglamd_fused_rms_row_quant(x.data_ptr(), stride, res ? res->data_ptr() : nullptr, res_stride, w.data_ptr(), (float)eps, o.fixed, rows,
+                                     hidden, o.q.data_ptr(), o.s.data_ptr<float>(), o.zero_points(), y ? y->data_ptr() : nullptr,
+                                     res_out ? res_out->data_ptr() : nullptr, tag(t), tag(w.scalar_type()), tag(q_dtype), stream_of(x)));
+  return {o.q, o.s, o.zp, y, res_out};
+}
+
+std::tuple<Tensor, Tensor, optional<Tensor>> silu_mul_row_quant(const Tensor& x, ScalarType q_dtype, bool symmetric, const optional<Tensor>& scale) {
+  refuse_observed("silu_and_mul_row_quant", x, scale);
+  const int64_t stride = row_stride(x, "input"), rows = x.size(0);
+  TORCH_CHECK(x.size(1) % 2 == 0, "input rows must be [gate | up]");
+  TORCH_CHECK(is_half(x.scalar_type()), "input must be Half or BFloat16");
+  const c10::DeviceGuard guard(x.device());
+  const RowCodes o(x, rows, x.size(1) / 2, q_dtype, symmetric, scale);
+  if (rows)
+    check(sglamd_silu_mul_row_quant(x.data_ptr(), stride, o.fixed, rows, x.size(1) / 2, o.q.data_ptr(), o.s.data_ptr<float>(), o.zero_points(),
+                                    tag(x.scalar_type()), tag(q_dtype), stream_of(x)));
+  return {o.q, o.s, o.zp};
+}
+
+std::tuple<Tensor, Tensor, Tensor> per_token_quant_int8_asym(const Tensor& x) {
+  refuse_observed("per_token_quant_int8_asym", x);
+  const int64_t stride = row_stride(x, "x"), rows = x.size(0), hidden = x.size(1);
+  const ScalarType t = x.scalar_type();
+  TORCH_CHECK(t == at::kFloat || is_half(t), "x must be Float, Half or BFloat16");
+  const c10::DeviceGuard guard(x.device());
+  const RowCodes o(x, rows, hidden, at::kChar, false, {});
+  if (rows)
+    check(sglamd_per_token_quant_int8_asym(x.data_ptr(), stride, tag(t), rows, hidden, (int8_t*)o.q.data_ptr(), o.s.data_ptr<float>(),
+                                           o.zero_points(), stream_of(x)));
+  return {o.q, o.s, *o.zp};
+}
+
+Tensor int8_weight_sums(const Tensor& weight) {
+  refuse_observed("int8_weight_sums", weight);
+  TORCH_CHECK(weight.dim() == 2 && weight.scalar_type() == at::kChar, "weight must be a 2D Int8 tensor");
+  TORCH_CHECK(weight.stride(0) == 1 || weight.size(0) <= 1, "weight must be the column-major [K, N] view of [N, K] rows");
+  const int64_t k = weight.size(0), n = weight.size(1);
+  const c10::DeviceGuard guard(weight.device());
+  const Tensor sums = empty({n}, at::kInt, weight);
+  if (n) check(sglamd_int8_weight_sums(weight.data_ptr(), ld(weight, 1), n, k, sums.data_ptr<int32_t>(), stream_of(weight)));
+  return sums;
+}
+
+// ---------------------------------------------------------------------------------------
 // dense GEMMs
 // ---------------------------------------------------------------------------------------
 // fp32 split-K scratch when the library can use one for this shape; from the caching allocator, so calls on other
@@ -541,6 +653,83 @@ Tensor int8_scaled_mm(const Tensor& a, const Tensor& b, const Tensor& sa, const 
   TORCH_CHECK(b.scalar_type() == at::kChar, "mat_b must be Int8");
   TORCH_CHECK(is_half(out_dtype), "out_dtype must be Half or BFloat16");
   return rowwise_mm(true, a, b, sa, sb, out_dtype, bias);
+}
+
+// One value for each of n rows or columns, on x's device.
+void check_vector(const Tensor& v, const Tensor& x, int64_t n, ScalarType t, const char* name) {
+  TORCH_CHECK(v.numel() == n, "size of ", name, " is not matched");
+  TORCH_CHECK(v.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(v.scalar_type() == t, name, " must be ", t);
+  check_same_device(v, x, name);
+}
+
+void check_int8_weight(const Tensor& x, const Tensor& b) {
+  TORCH_CHECK(b.scalar_type() == at::kChar, "mat_b must be Int8");
+  check_same_device(b, x, "mat_b");
+  TORCH_CHECK(b.size(0) % 16 == 0, "mat_b.size(0) must be multiple of 16 for memory alignment");
+  TORCH_CHECK(b.size(1) % 8 == 0, "mat_b.size(1) must be multiple of 8 for memory alignment");
+}
+
+// int8_scaled_mm of rows with a zero point each: (a - azp) x b, `sums` the weight's sums over K
+Tensor int8_scaled_mm_azp(const Tensor& a, const Tensor& b, const Tensor& sa, const Tensor& sb, ScalarType out_dtype, const Tensor& azp,
+                          const Tensor& sums, const optional<Tensor>& bias) {
+  refuse_observed("int8_scaled_mm_azp", a, b, sa, sb, azp, sums, bias);
+  check_mm_operands(a, b);
+  TORCH_CHECK(a.scalar_type() == at::kChar, "mat_a must be Int8");
+  check_int8_weight(a, b);
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(1);
+  check_vector(sa, a, m, at::kFloat, "scales_a");
+  check_vector(sb, a, n, at::kFloat, "scales_b");
+  check_vector(azp, a, m, at::kInt, "azp");
+  check_vector(sums, a, n, at::kInt, "weight_sums");
+  TORCH_CHECK(is_half(out_dtype), "out_dtype must be Half or BFloat16");
+  if (bias) check_vector(*bias, a, n, out_dtype, "bias");
+  const c10::DeviceGuard guard(a.device());
+  Tensor out = empty({m, n}, out_dtype, a);
+  if (m == 0 || n == 0) return out;
+  void* wp;
+  int64_t wb;
+  const Tensor ws = gemm_workspace(m, n, k, true, a, &wp, &wb);
+  check(sglamd_int8_scaled_mm_azp(a.data_ptr(), ld(a, 0), b.data_ptr(), ld(b, 1), sa.data_ptr<float>(), sb.data_ptr<float>(),
+                                  azp.data_ptr<int32_t>(), sums.data_ptr<int32_t>(), bias ? bias->data_ptr() : nullptr, out.data_ptr(), n,
+                                  tag(out_dtype), m, n, k, wp, wb, stream_of(a)));
+  return out;
+}
+
+// A linear layer on int8 weights with a scale per channel: x quantised per token, with zero points where the weight's sums are
+// given, then the product.  One allocation beside the output.
+Tensor int8_linear(const Tensor& x, const Tensor& weight, const Tensor& ws, const optional<Tensor>& sums, const optional<Tensor>& bias) {
+  refuse_observed("apply_int8_linear", x, weight, ws, sums, bias);
+  check_mm_operands(x, weight);
+  const ScalarType t = x.scalar_type();
+  TORCH_CHECK(is_half(t), "input must be Half or BFloat16");
+  check_int8_weight(x, weight);
+  const int64_t m = x.size(0), k = x.size(1), n = weight.size(1);
+  check_vector(ws, x, n, at::kFloat, "weight_scale");
+  if (sums) check_vector(*sums, x, n, at::kInt, "weight_sums");
+  if (bias) check_vector(*bias, x, n, t, "bias");
+  const c10::DeviceGuard guard(x.device());
+  Tensor out = empty({m, n}, t, x);
+  if (m == 0 || n == 0) return out;
+  TORCH_CHECK(k > 0, "rows must not be empty");
+  Scratch sc;
+  const int64_t q = sc.take(m * k), sa = sc.take(4 * m), zp = sums ? sc.take(4 * m) : 0;
+  const int64_t wb = sglamd_gemm_workspace_bytes(m, n, k), wp = sc.take(wb > 0 ? wb : 0);
+  sc.allocate(x);
+  void* st = stream_of(x);
+  void* wsp = wb > 0 ? sc.at(wp) : nullptr;
+  if (sums) {
+    check(sglamd_per_token_quant_int8_asym(x.data_ptr(), ld(x, 0), tag(t), m, k, (int8_t*)sc.at(q), (float*)sc.at(sa), (int32_t*)sc.at(zp), st));
+    check(sglamd_int8_scaled_mm_azp(sc.at(q), k, weight.data_ptr(), ld(weight, 1), (float*)sc.at(sa), ws.data_ptr<float>(),
+                                    (int32_t*)sc.at(zp), sums->data_ptr<int32_t>(), bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, tag(t),
+                                    m, n, k, wsp, wb, st));
+    return out;
+  }
+  const Tensor rows = x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
+  check(sglamd_per_token_quant_int8(rows.data_ptr(), tag(t), (int8_t*)sc.at(q), (float*)sc.at(sa), m, k, st));
+  check(sglamd_int8_scaled_mm(sc.at(q), k, weight.data_ptr(), ld(weight, 1), (float*)sc.at(sa), ws.data_ptr<float>(),
+                              bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, tag(t), m, n, k, wsp, wb, st));
+  return out;
 }
 
 bool plain_weight(const Tensor& w, const Tensor& x, ScalarType t) {
@@ -1095,6 +1284,48 @@ optional<Tensor> moe_layer(const Tensor& hidden, const Tensor& w1, const Tensor&
   return out;
 }
 
+// The expert layer of a few tokens in 8 bits (moe_runner/few_tokens.py states the contract)
+Tensor experts_few_tokens(const Tensor& x, const Tensor& xs, const Tensor& w1, const Tensor& w2, const Tensor& s1, const Tensor& s2,
+                          const Tensor& weights, const Tensor& ids, ScalarType out_dtype, const optional<Tensor>& b1,
+                          const optional<Tensor>& b2, double factor) {
+  const char* op = "fused_experts_few_tokens";
+  refuse_observed(op, x, xs, w1, w2, s1, s2, weights, ids, b1, b2);
+  check_input(x, "hidden_q");
+  const ScalarType qt = x.scalar_type();
+  TORCH_CHECK(x.dim() == 2 && (qt == kFp8 || qt == at::kChar), "hidden_q must be 2D, Float8_e4m3fn or Char");
+  const int64_t m = x.size(0), h = x.size(1);
+  TORCH_CHECK(w1.dim() == 3 && w2.dim() == 3 && w1.is_contiguous() && w2.is_contiguous() && w1.scalar_type() == qt && w2.scalar_type() == qt,
+              "expert weights must be contiguous 3D tensors of the rows' dtype");
+  const int64_t e = w1.size(0), n2 = w1.size(1), i = n2 / 2;
+  TORCH_CHECK(n2 % 2 == 0 && w1.size(2) == h && w2.size(0) == e && w2.size(1) == h && w2.size(2) == i,
+              "w1 must be [E, 2 * intermediate, hidden] and w2 [E, hidden, intermediate]");
+  check_same_device(w1, x, "w1");
+  check_same_device(w2, x, "w2");
+  check_vector(xs, x, m, at::kFloat, "hidden_scale");
+  check_vector(s1, x, e * n2, at::kFloat, "w1_scale");
+  check_vector(s2, x, e * h, at::kFloat, "w2_scale");
+  TORCH_CHECK(is_half(out_dtype), "out_dtype must be Half or BFloat16");
+  if (b1) check_vector(*b1, x, e * n2, out_dtype, "b1");
+  if (b2) check_vector(*b2, x, e * h, out_dtype, "b2");
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == m && ids.sizes() == weights.sizes(), "topk_weights and topk_ids must be [tokens, topk]");
+  TORCH_CHECK(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, "topk_ids must be int32/int64");
+  check_same_device(ids, x, "topk_ids");
+  check_same_device(weights, x, "topk_weights");
+  const int64_t topk = ids.size(1);
+  const c10::DeviceGuard guard(x.device());
+  Tensor out = empty({m, h}, out_dtype, x);
+  if (m == 0) return out;
+  const Tensor tw = weights.to(at::kFloat).contiguous(), at_ids = ids.contiguous();
+  const int64_t need = sglamd_fused_experts_few_tokens_workspace(m, i, (int)std::min<int64_t>(topk, 1 << 20));
+  const Tensor ws = empty({std::max<int64_t>(need, 16)}, at::kByte, x);
+  check(sglamd_fused_experts_few_tokens(x.data_ptr(), xs.data_ptr<float>(), tag(qt), m, h, i, (int)std::min<int64_t>(e, 0x7fffffff),
+                                        (int)std::min<int64_t>(topk, 1 << 20), w1.data_ptr(), s1.data_ptr<float>(), b1 ? b1->data_ptr() : nullptr,
+                                        w2.data_ptr(), s2.data_ptr<float>(), b2 ? b2->data_ptr() : nullptr, tw.data_ptr<float>(),
+                                        at_ids.data_ptr(), tag(at_ids.scalar_type()), out.data_ptr(), tag(out_dtype), (float)factor, ws.data_ptr(),
+                                        need, stream_of(x)));
+  return out;
+}
+
 // cutlass_fused_experts_fp8 (cutlass_moe.py:29-341) in its block-scaled configuration: w1 [E, k, 2n] and w2 [E, n, k] as
 // column-major views of contiguous [E, 2n, k] / [E, k, n] weights, the scales as the matching views.
 optional<Tensor> moe_grouped_layer(const Tensor& a, const Tensor& w1, const Tensor& w2, const Tensor& w1_scale,
@@ -1230,6 +1461,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_quant_2d", &group_quant_2d, Unlocked());
   m.def("per_token_quant", &per_token_quant, Unlocked());
   m.def("fused_rms_group_quant", &fused_rms_group_quant, Unlocked());
+  m.def("fused_rms_row_quant", &fused_rms_row_quant, Unlocked());
+  m.def("silu_mul_row_quant", &silu_mul_row_quant, Unlocked());
+  m.def("per_token_quant_int8_asym", &per_token_quant_int8_asym, Unlocked());
+  m.def("int8_weight_sums", &int8_weight_sums, Unlocked());
+  m.def("int8_scaled_mm_azp", &int8_scaled_mm_azp, Unlocked());
+  m.def("int8_linear", &int8_linear, Unlocked());
+  m.def("experts_few_tokens", &experts_few_tokens, Unlocked());
   m.def("w8a8_block_fp8_matmul_", &w8a8_block_fp8_matmul_, Unlocked(), py::arg("A"), py::arg("B"), py::arg("As"), py::arg("Bs"),
         py::arg("C"), py::arg("pow2_scales") = false);
   m.def("w8a8_block_int8_matmul_", &w8a8_block_int8_matmul_, Unlocked());

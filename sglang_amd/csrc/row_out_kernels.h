@@ -1,0 +1,226 @@
+// The kernels of row_out.h, instantiated by row_norm.hip (RMSNorm) and row_act.hip (SiLU * up, plain rows).
+#pragma once
+#include "row_out.h"
+
+namespace sglamd {
+
+// Eight values of a lane's piece `i` (0: a row of zeros past its end).
+template <typename T>
+__device__ __forceinline__ void unpack8(const v4i& raw, float* out) {
+  u16 b[8];
+  __builtin_memcpy(b, &raw, 16);
+#pragma unroll
+  for (int j = 0; j < 8; j++) out[j] = T::to_f32(b[j]);
+}
+template <typename T>
+__device__ __forceinline__ v4i pack8(const float* v) {
+  return v4i{(int)T::pack2(v[0], v[1]), (int)T::pack2(v[2], v[3]), (int)T::pack2(v[4], v[5]), (int)T::pack2(v[6], v[7])};
+}
+// exp by the hardware's exp2 and a reciprocal of 1 ulp each: relative error of some 2^-23 * (2 + |gate|), the second part only
+// on gates so negative that the value is lost beside the row's largest
+__device__ __forceinline__ float silu_mul(float gate, float up) {
+  const float t = __builtin_amdgcn_exp2f(gate * -1.44269504088896340736f);
+  return gate * __builtin_amdgcn_rcpf(1.0f + t) * up;
+}
+
+// A row's lanes: TEAM = 64, one wave (no barrier), or 0, the workgroup.  Each holds NV pieces of 8 values.
+template <typename T, typename WT, int SRC, int QK, int NV, int TEAM>
+__device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t row, uint32_t* red) {
+  const int nt = TEAM ? TEAM : (int)blockDim.x, tid = TEAM ? (int)threadIdx.x & 63 : (int)threadIdx.x;
+  const int nvec = row < a.rows ? (int)(a.hidden >> 3) : 0;
+  const u16* x = (const u16*)a.x + row * a.x_stride;
+  const v4i zero = {0, 0, 0, 0};
+
+  // every load of the row is requested before the first is used
+  v4i raw[NV], second[SRC == ROW_PLAIN ? 1 : NV], wraw[SRC == ROW_RMS ? NV : 1][sizeof(typename WT::storage) == 4 ? 2 : 1];
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    const int i = tid + k * nt;
+    const bool live = i < nvec;
+    raw[k] = live ? *((const v4i*)x + i) : zero;
+    if constexpr (SRC == ROW_SILU) second[k] = live ? *((const v4i*)(x + a.hidden) + i) : zero;
+    if constexpr (SRC == ROW_RMS) {
+      second[k] = live && a.res ? *((const v4i*)((const u16*)a.res + row * a.res_stride) + i) : zero;
+      if constexpr (sizeof(typename WT::storage) == 4) {
+        wraw[k][0] = live ? *((const v4i*)a.w + 2 * i) : zero;
+        wraw[k][1] = live ? *((const v4i*)a.w + 2 * i + 1) : zero;
+      } else {
+        wraw[k][0] = live ? *((const v4i*)a.w + i) : zero;
+      }
+    }
+  }
+
+  float u[NV][8];
+  RowStats t = {0.f, 0u, 0u};
+  float poison = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    unpack8<T>(raw[k], u[k]);
+    if constexpr (SRC == ROW_SILU) {
+      float up[8];
+      unpack8<T>(second[k], up);
+#pragma unroll
+      for (int j = 0; j < 8; j++) u[k][j] = silu_mul(u[k][j], up[j]);
+    }
+    if constexpr (SRC == ROW_RMS) {
+      if (a.res) {
+        float r[8];
+        unpack8<T>(second[k], r);
+#pragma unroll
+        for (int j = 0; j < 8; j++) u[k][j] += r[j];
+        const int i = tid + k * nt;
+        if (i < nvec) *((v4i*)((u16*)a.res_out + row * a.hidden) + i) = pack8<T>(u[k]);
+      }
+      float w[8];
+      if constexpr (sizeof(typename WT::storage) == 4) {
+        __builtin_memcpy(w, wraw[k], 32);
+      } else {
+        unpack8<WT>(wraw[k][0], w);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        t.ss = fmaf(u[k][j], u[k][j], t.ss);
+        u[k][j] *= w[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      row_stats_add<SRC, QK>(t, u[k][j]);
+      if (QK == ROW_TO_ASYM && SRC != ROW_RMS) poison = fmaf(u[k][j], 0.f, poison);
+    }
+  }
+  if (QK == ROW_TO_ASYM && SRC != ROW_RMS) row_stats_poison(t, poison);
+  t = TEAM ? row_stats_wave<SRC, QK>(t) : row_stats_block<SRC, QK>(t, red);
+  const RowScale o = row_scale<SRC, QK>(a, t);
+  if (row >= a.rows) return;
+  if (tid == 0) {
+    a.s[row] = o.scale;
+    if (QK == ROW_TO_ASYM) a.zp[row] = (int32_t)o.zp;
+  }
+  uint8_t* q = a.q + row * a.hidden;
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    const int i = tid + k * nt;
+    if (i >= nvec) break;
+    *((v2i*)q + i) = v2i{(int)row_codes4<QK>(u[k], o), (int)row_codes4<QK>(u[k] + 4, o)};
+    if (SRC == ROW_RMS && a.y) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = u[k][j] * o.r;
+      *((v4i*)((u16*)a.y + row * a.hidden) + i) = pack8<T>(y);
+    }
+  }
+}
+
+template <typename T, typename WT, int SRC, int QK, int NT, int NV>
+__global__ __launch_bounds__(NT) void row_out_kernel(RowOutArgs a) {
+  __shared__ uint32_t red[48];
+  row_out_body<T, WT, SRC, QK, NV, 0>(a, blockIdx.x, red);
+}
+// Short rows, a wave each.
+template <typename T, typename WT, int SRC, int QK, int NV>
+__global__ __launch_bounds__(256) void row_out_team_kernel(RowOutArgs a) {
+  row_out_body<T, WT, SRC, QK, NV, 64>(a, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), nullptr);
+}
+
+// Any row length and alignment, 32-bit rows: a workgroup per row, values one by one, the row read twice (the second time
+// from L2).
+template <typename T, typename WT, int SRC, int QK>
+__global__ __launch_bounds__(256) void row_out_any_kernel(RowOutArgs a) {
+  typedef typename T::storage S;
+  __shared__ uint32_t red[48];
+  const int64_t row = blockIdx.x;
+  const S* x = (const S*)a.x + row * a.x_stride;
+  const S* res = a.res ? (const S*)a.res + row * a.res_stride : nullptr;
+  auto sum_at = [&](int64_t i) -> float { return T::to_f32(x[i]) + (res ? T::to_f32(res[i]) : 0.f); };
+  auto value_at = [&](int64_t i) -> float {
+    if constexpr (SRC == ROW_RMS) return sum_at(i) * WT::to_f32(((const typename WT::storage*)a.w)[i]);
+    else if constexpr (SRC == ROW_SILU) return silu_mul(T::to_f32(x[i]), T::to_f32(x[a.hidden + i]));
+    else return T::to_f32(x[i]);
+  };
+  RowStats t = {0.f, 0u, 0u};
+  float poison = 0.f;
+  for (int64_t i = threadIdx.x; i < a.hidden; i += 256) {
+    if constexpr (SRC == ROW_RMS) {
+      const float v = sum_at(i);
+      t.ss = fmaf(v, v, t.ss);
+      if (res) ((S*)a.res_out)[row * a.hidden + i] = T::from_f32(v);
+    }
+    const float u = value_at(i);
+    row_stats_add<SRC, QK>(t, u);
+    if (QK == ROW_TO_ASYM && SRC != ROW_RMS) poison = fmaf(u, 0.f, poison);
+  }
+  if (QK == ROW_TO_ASYM && SRC != ROW_RMS) row_stats_poison(t, poison);
+  t = row_stats_block<SRC, QK>(t, red);
+  const RowScale o = row_scale<SRC, QK>(a, t);
+  if (threadIdx.x == 0) {
+    a.s[row] = o.scale;
+    if (QK == ROW_TO_ASYM) a.zp[row] = (int32_t)o.zp;
+  }
+  for (int64_t i = threadIdx.x; i < a.hidden; i += 256) {
+    float v[4] = {value_at(i), 0.f, 0.f, 0.f};
+    a.q[row * a.hidden + i] = (uint8_t)row_codes4<QK>(v, o);
+    if (SRC == ROW_RMS && a.y) ((S*)a.y)[row * a.hidden + i] = T::from_f32(v[0] * o.r);
+  }
+}
+
+constexpr int64_t ROW_OUT_MAX_HIDDEN = 1024 * 8 * 4;  // the longest row that 1024 lanes keep in registers
+
+template <typename T, typename WT, int SRC, int QK>
+static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
+  const dim3 grid((unsigned)a.rows);
+  if (!pieces) {
+    hipLaunchKernelGGL((row_out_any_kernel<T, WT, SRC, QK>), grid, dim3(256), 0, st, a);
+    return;
+  }
+  if constexpr (sizeof(typename T::storage) == 2) {
+    const int64_t nvec = a.hidden >> 3;
+    const bool many = a.rows >= 2 * (int64_t)device_cus();
+    if (many && nvec <= 128) {
+      const dim3 teams((unsigned)ceil_div(a.rows, 4));
+      if (nvec <= 64) hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, 1>), teams, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, 2>), teams, dim3(256), 0, st, a);
+      return;
+    }
+#define SGLAMD_ROW_OUT(NT, NV) hipLaunchKernelGGL((row_out_kernel<T, WT, SRC, QK, NT, NV>), grid, dim3(NT), 0, st, a)
+    if (nvec <= 256) SGLAMD_ROW_OUT(256, 1);
+    else if (many && nvec <= 512) SGLAMD_ROW_OUT(256, 2);
+    else if (many && nvec <= 1024) SGLAMD_ROW_OUT(256, 4);
+    else if (nvec <= 1024) SGLAMD_ROW_OUT(1024, 1);
+    else if (nvec <= 2048) SGLAMD_ROW_OUT(1024, 2);
+    else SGLAMD_ROW_OUT(1024, 4);
+#undef SGLAMD_ROW_OUT
+  }
+}
+template <typename T, typename WT, int SRC>
+static int launch_row_out_to(const RowOutArgs& a, int q_kind, bool pieces, hipStream_t st) {
+  if (q_kind == ROW_TO_FP8) launch_row_out<T, WT, SRC, ROW_TO_FP8>(a, pieces, st);
+  else if (q_kind == ROW_TO_INT8) launch_row_out<T, WT, SRC, ROW_TO_INT8>(a, pieces, st);
+  else launch_row_out<T, WT, SRC, ROW_TO_ASYM>(a, pieces, st);
+  return check_launch("row_out");
+}
+
+// What every entry point asks of its rows and outputs.
+static inline int check_row_out(const char* op, const RowOutArgs& a, int64_t width, int q_dtype) {
+  SGLAMD_REQUIRE(a.x && a.q && a.s, SGLAMD_EINVAL, "%s: null pointer", op);
+  SGLAMD_REQUIRE(a.rows >= 0 && a.rows < (1ll << 31) && a.hidden > 0 && a.hidden < (1ll << 31), SGLAMD_EINVAL,
+                 "%s: bad sizes (%lld rows of %lld)", op, (long long)a.rows, (long long)a.hidden);
+  SGLAMD_REQUIRE(a.x_stride >= 0 && (a.x_stride >= width || a.x_stride == 0), SGLAMD_EINVAL,
+                 "%s: row stride %lld is smaller than the row (%lld)", op, (long long)a.x_stride, (long long)width);
+  SGLAMD_REQUIRE(q_dtype == SGLAMD_FP8_E4M3 || q_dtype == SGLAMD_I8, SGLAMD_EINVAL, "%s: the codes must be FP8_E4M3 or I8", op);
+  SGLAMD_REQUIRE(!a.zp || q_dtype == SGLAMD_I8, SGLAMD_EINVAL, "%s: zero points go with I8 codes", op);
+  SGLAMD_REQUIRE(!a.fixed || q_dtype == SGLAMD_FP8_E4M3, SGLAMD_ENOTSUP, "%s: a given scale goes with FP8_E4M3 codes", op);
+  return SGLAMD_OK;
+}
+static inline int row_out_kind(const RowOutArgs& a, int q_dtype) {
+  return q_dtype == SGLAMD_FP8_E4M3 ? ROW_TO_FP8 : a.zp ? ROW_TO_ASYM : ROW_TO_INT8;
+}
+static inline bool aligned_to(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+// Whether the rows can be taken in pieces of 8 values, 16 bytes in and 8 out, and kept in registers.
+static inline bool row_out_pieces(const RowOutArgs& a) {
+  return a.hidden % 8 == 0 && a.hidden <= ROW_OUT_MAX_HIDDEN && a.x_stride % 8 == 0 && aligned_to(a.x, 16) && aligned_to(a.q, 8) &&
+         (!a.res || (a.res_stride % 8 == 0 && aligned_to(a.res, 16) && aligned_to(a.res_out, 16))) && (!a.w || aligned_to(a.w, 16)) &&
+         (!a.y || aligned_to(a.y, 16));
+}
+
+}  // namespace sglamd

@@ -24,6 +24,16 @@ def per_token_quant_int8(x: torch.Tensor, scale_dtype=torch.float32, cal_sum: bo
     return x_q, scales
 
 
+def per_token_quant_int8_asym(x: torch.Tensor):
+    """(x_q int8 like x, scales float32 [..., 1], zero points int32 [..., 1]) with x about scale * (x_q - zp): the whole int8
+    range over [min(0, min x), max(0, max x)] of each row (the formulas are those of fused_row_quant).  x float32, half or
+    bfloat16 [..., hidden]; 2D inputs may have any row stride."""
+    if x.dim() != 2:
+        assert x.is_contiguous()
+    q, s, zp = _C.per_token_quant_int8_asym(x if x.dim() == 2 else x.view(-1, x.shape[-1]))
+    return (q, s, zp) if x.dim() == 2 else (q.view(x.shape), s.view(x.shape[:-1] + (1,)), zp.view(x.shape[:-1] + (1,)))
+
+
 def per_token_group_quant_int8(x: torch.Tensor, group_size: int, eps: float = 1e-10, dtype: torch.dtype = torch.int8):
     """Per-token-group INT8 quantisation (int8_kernel.py:134-190): x [..., hidden] contiguous ->
     (x_q int8 like x, x_s fp32 [..., hidden // group_size]); scale = max(absmax, eps) / 127."""
