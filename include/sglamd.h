@@ -480,7 +480,7 @@ int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_stride, int dt
  * x [M, H] e4m3fn or int8 (q_dtype), contiguous; w13 [E, 2 * I, H] (gate rows, then up rows), w2 [E, H, I] of that type;
  * w13_scale fp32 [E, 2 * I], w2_scale [E, H]; b13, b2 optional, shaped like the scales, in out_dtype (F16/BF16);
  * topk_weights fp32 [M, topk], topk_ids [M, topk] int32 or int64: pairs whose id is outside [0, E) contribute nothing, an
- * id may be named more than once.  H and I multiples of 16, I <= 16384, M * topk <= 64 (more: SGLAMD_ENOTSUP).  workspace:
+ * id may be named more than once.  H and I multiples of 16, H <= 32768, I <= 16384, M * topk <= 64 (more: SGLAMD_ENOTSUP).  workspace:
  * sglamd_fused_experts_few_tokens_workspace(...) bytes, 16-byte aligned, nothing in it has to start at zero; calls that
  * overlap need workspaces of their own. */
 int64_t sglamd_fused_experts_few_tokens_workspace(int64_t M, int64_t I, int topk);

@@ -9,12 +9,23 @@
 // every e4m3 number, in v_dot2_f32_f16), at a few instructions per weight byte where the memory delivers ten bytes per
 // clock to a CU.  So nothing is staged: LPR lanes read LPR * 16 contiguous bytes of a weight row, the weights go straight
 // from memory into the registers of the lanes that multiply them, and LPR lanes add up at the end of a row.
-//   * Pairs that name the same expert are one group: its weights are read once for up to R rows.  Groups are found from the
+//   * Pairs that name the same expert are one group: its weights are read once for up to RMAX rows.  Groups are found from the
 //     ids by ballots, by every wave for itself, so there is no sorting launch and nothing to clear.
 //   * First launch: a wave owns 64 / LPR columns of one group, gate row and up row side by side, and writes a.
 //   * Second launch: a workgroup owns 2 * 64 / LPR output columns and ALL pairs, a group to a wave in turn.  A wave quantises
-//     the rows of its group itself, while its first weights are on their way; the pairs' results meet in LDS and are summed
-//     in the pairs' order, so the sum over a token's experts needs neither atomics nor a launch.
+//     the rows of its group itself, in front of which it has requested its first weights; the pairs' results meet in LDS and
+//     are summed in the pairs' order, so the sum over a token's experts needs neither atomics nor a launch.
+//
+// Measured (kernels, us; in brackets a bare read of the weights' bytes): 6 of 64 int8 experts of 4096 x 1536, one token, 15.2 + 10.6
+// (16.4); 8 of 128 e4m3 experts of 2048 x 768, three tokens, 15.1 + 14.7 (15.5); 8 of 256 of 7168 x 2048, one token 38.7 + 23.2 (51),
+// four 133 + 80 (195).  Large layers run at the rate of a read; small ones wait for two launches, and in each for a chain of ids, rows
+// and first weights, some 4 us a launch.
+// Tried: the second launch's rows quantised by the workgroup together, behind a barrier (four tokens of the large layer 80 -> 89: all
+// waves quantise at once and all stream at once); sixteen waves to its workgroups (registers spill, 14 -> 22); a wave's next group
+// requested under the results of the one before (80 -> 97 where it spills, 78 -> 80 elsewhere); the first launch's rows from L1 instead of LDS
+// (their loads return behind the weights that were requested before them: 4096 x 1408, four tokens, 20.6 against 13.3).
+#include <algorithm>
+
 #include "row_out.h"
 
 namespace sglamd {
@@ -35,7 +46,9 @@ struct FewArgs {
 };
 
 constexpr int FEW_MAX_PAIRS = 64;  // one lane each
-constexpr int FEW_MAX_INTER = 16384;
+constexpr int FEW_MAX_HIDDEN = 32768, FEW_MAX_INTER = 16384;  // a row in LDS, eight of them
+constexpr int FEW_DOWN_WAVES = 8;
+constexpr int FEW_LDS = 64 * 1024;  // what several rows for a pass may take, two workgroups to a CU
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
@@ -65,55 +78,83 @@ __device__ __forceinline__ void dot16(const v4i& w0, const v4i& w1, const v4i (&
   }
 }
 
-// A batch of S steps of LPR * 16 bytes of two weight rows, per lane.
+// A batch of S steps of LPR * 16 bytes of two weight rows, per lane.  The loads of a batch are straight-line code, and the next
+// batch is requested without a condition: at a join of two paths the compiler could not tell how many loads are newer than the
+// ones it waits for, and would wait for all (a conditional request cost a tenth of a layer of 64 experts of 4096 x 1536).
+// Steps of a batch: two; four where several rows share a pass in a large layer (7168 x 2048, four tokens, 137 + 83 -> 133 + 80; one token of
+// 4096 x 1536 with four 16.4 instead of 15.2).
+constexpr int few_batch(int rmax, int lpr) { return rmax > 1 && lpr == 8 ? 4 : 2; }
 template <int S>
 struct FewBatch {
   v4i w0[S], w1[S];
 };
 template <int S, int LPR>
-__device__ __forceinline__ FewBatch<S> few_load(const uint8_t* w0, const uint8_t* w1, int step) {
-  FewBatch<S> b;
+__device__ __forceinline__ void few_load(FewBatch<S>& b, const uint8_t* w0, const uint8_t* w1, int step) {
 #pragma unroll
   for (int s = 0; s < S; s++) {
-    b.w0[s] = load_once(w0 + (int64_t)(step + s) * (LPR * 16));
-    b.w1[s] = load_once(w1 + (int64_t)(step + s) * (LPR * 16));
+    b.w0[s] = load_once(w0 + (step + s) * (LPR * 16));
+    b.w1[s] = load_once(w1 + (step + s) * (LPR * 16));
   }
-  return b;
+}
+// The batch that ends a row of K codes: pieces past its end are fetched from its last one and replaced by zeros.  (Behind zero
+// weights the rows' codes are fetched from there too: only a row that holds a NaN multiplies one by a zero.)
+template <int LPR>
+__device__ __forceinline__ int few_piece(int step, int K, int sub) { return min(step * (LPR * 16), K - 16 - sub * 16); }
+template <int S, int LPR>
+__device__ __forceinline__ void few_load_last(FewBatch<S>& b, const uint8_t* w0, const uint8_t* w1, int step, int K, int sub) {
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    const int at = few_piece<LPR>(step + s, K, sub);
+    b.w0[s] = load_once(w0 + at);
+    b.w1[s] = load_once(w1 + at);
+  }
+}
+template <int S, int LPR>
+__device__ __forceinline__ void few_load_first(FewBatch<S>& b, const uint8_t* w0, const uint8_t* w1, int K, int sub) {
+  if (S * (LPR * 16) <= K) few_load<S, LPR>(b, w0, w1, 0);
+  else few_load_last<S, LPR>(b, w0, w1, 0, K, sub);
 }
 
-// acc over a whole row of K codes.  w0, w1: the lane's piece of the first step; fetch(step, r): its piece of row r; `first`: the
-// first batch where there is one (K / (LPR * 16) >= S).
+// acc over a whole row of K codes.  w0, w1: the lane's piece of the first step, `cur` the first batch; fetch(offset, r): the lane's
+// piece of row r, `offset` bytes behind that of its first step.
 template <bool INT8, int R, int LPR, int S, typename A, typename F>
-__device__ __forceinline__ void few_dot(const uint8_t* w0, const uint8_t* w1, int K, int sub, const FewBatch<S>& first, F fetch, A (&acc)[2][R]) {
-  const int full = K / (LPR * 16);
-  int i = 0;
-  FewBatch<S> cur = first;
-  for (; i + S <= full; i += S) {
-    FewBatch<S> next = cur;
-    if (i + 2 * S <= full) next = few_load<S, LPR>(w0, w1, i + S);
-    v4i x[S][R];
+__device__ __forceinline__ void few_dot(const uint8_t* w0, const uint8_t* w1, int K, int sub, FewBatch<S>& cur, F fetch, A (&acc)[2][R]) {
+  const int full = K / (LPR * 16), steps = (K + LPR * 16 - 1) / (LPR * 16);
+  auto consume = [&](const FewBatch<S>& b, int i) {
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      v4i x[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) x[r] = fetch((i + s) * (LPR * 16), r);
+      dot16<INT8, R>(b.w0[s], b.w1[s], x, acc);
+    }
+  };
+  auto consume_last = [&](const FewBatch<S>& b, int i) {
 #pragma unroll
     for (int s = 0; s < S; s++)
+      if (i + s < steps) {
+        const v4i zero = {0, 0, 0, 0};
+        const bool live = (i + s) * (LPR * 16) + sub * 16 < K;
+        v4i x[R];
 #pragma unroll
-      for (int r = 0; r < R; r++) x[s][r] = fetch(i + s, r);
-#pragma unroll
-    for (int s = 0; s < S; s++) dot16<INT8, R>(cur.w0[s], cur.w1[s], x[s], acc);
-    cur = next;
-  }
-  // single steps, the last of them with lanes past the end of the row
-  for (; i * (LPR * 16) < K; i++) {
-    const bool live = i * (LPR * 16) + sub * 16 < K;
-    v4i x[R], a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-#pragma unroll
-    for (int r = 0; r < R; r++) x[r] = v4i{0, 0, 0, 0};
-    if (live) {
-      a = load_once(w0 + (int64_t)i * (LPR * 16));
-      b = load_once(w1 + (int64_t)i * (LPR * 16));
-#pragma unroll
-      for (int r = 0; r < R; r++) x[r] = fetch(i, r);
+        for (int r = 0; r < R; r++) x[r] = fetch(few_piece<LPR>(i + s, K, sub), r);
+        dot16<INT8, R>(live ? b.w0[s] : zero, live ? b.w1[s] : zero, x, acc);
+        }
+  };
+  FewBatch<S> next;
+  int i = 0;
+  if (S <= full) {
+    for (; i + 2 * S <= full; i += S) {
+      few_load<S, LPR>(next, w0, w1, i + S);
+      consume(cur, i);
+      cur = next;
     }
-    dot16<INT8, R>(a, b, x, acc);
+    few_load_last<S, LPR>(next, w0, w1, min(i + S, steps - 1), K, sub);  // (where nothing is left, the last step again)
+    consume(cur, i);
+    cur = next;
+    i += S;
   }
+  if (i < steps) consume_last(cur, i);
 }
 
 // Sum over each aligned group of LPR lanes, in all of them.
@@ -154,6 +195,11 @@ __device__ __forceinline__ void few_groups(const FewArgs& a, F body) {
     if (!body(group, expert, members)) return;
   }
 }
+// The rows of a group that are still to be multiplied (0: none).
+struct FewGroup {
+  int expert;
+  unsigned long long members;
+};
 // The next R members; pairs[] beyond their number repeat the first.
 template <int R>
 __device__ __forceinline__ int few_take(unsigned long long& members, int (&pairs)[R]) {
@@ -166,81 +212,82 @@ __device__ __forceinline__ int few_take(unsigned long long& members, int (&pairs
   }
   return n;
 }
-template <int R>
-__device__ __forceinline__ float few_pick(const float (&v)[R], int r) {
-  float o = v[0];
-#pragma unroll
-  for (int j = 1; j < R; j++) o = r == j ? v[j] : o;
-  return o;
-}
-
-template <bool INT8, typename OT, int R, int LPR, int S>
-__device__ __forceinline__ void few_up_rows(const FewArgs& a, int expert, unsigned long long& members, int col, int sub) {
+// grid: column tiles of 4 waves x pairs (the groups are at most as many).  LDS: RMAX rows of H codes.
+template <bool INT8, typename OT, int RMAX, int LPR>
+__global__ __launch_bounds__(256) void few_up_kernel(FewArgs a) {
   typedef typename std::conditional<INT8, int, float>::type acc_t;
-  const int n = min(col, a.I - 1);
-  const int64_t gate_row = (int64_t)expert * 2 * a.I + n, up_row = gate_row + a.I;
-  const uint8_t* w0 = a.w + gate_row * a.H + sub * 16;
-  const uint8_t* w1 = a.w + up_row * a.H + sub * 16;
-  FewBatch<S> first = {};
-  if (a.H / (LPR * 16) >= S) first = few_load<S, LPR>(w0, w1, 0);
-  int pairs[R];
-  const int count = few_take<R>(members, pairs);
-  const uint8_t* x[R];
-#pragma unroll
-  for (int r = 0; r < R; r++) x[r] = a.x + (int64_t)(pairs[r] / a.topk) * a.H + sub * 16;
+  constexpr int S = few_batch(RMAX, LPR);
+  extern __shared__ __attribute__((aligned(16))) uint8_t rows[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LPR;
+  const int col = ((int)blockIdx.x * 4 + wave) * (64 / LPR) + lane / LPR;
+  FewGroup g = {0, 0};
+  few_groups(a, [&](int group, int expert, unsigned long long members) {
+    if (group == (int)blockIdx.y) g = {expert, members};
+    return group != (int)blockIdx.y;
+  });
+  if (!g.members) return;  // (the same for the whole workgroup)
+  const int64_t gate_row = (int64_t)g.expert * 2 * a.I + min(col, a.I - 1), up_row = gate_row + a.I;
+  const uint8_t *w0 = a.w + gate_row * a.H + sub * 16, *w1 = a.w + up_row * a.H + sub * 16;
   const float sg = a.s[gate_row], su = a.s[up_row];
   float bg = 0.f, bu = 0.f;
   if (a.b) {
     bg = OT::to_f32(((const typename OT::storage*)a.b)[gate_row]);
     bu = OT::to_f32(((const typename OT::storage*)a.b)[up_row]);
   }
-  acc_t acc[2][R] = {};
-  few_dot<INT8, R, LPR, S>(w0, w1, a.H, sub, first, [&](int step, int r) { return *(const v4i*)(x[r] + (int64_t)step * (LPR * 16)); }, acc);
-  float v[R];
+  for (;;) {
+    FewBatch<S> batch;
+    few_load_first<S, LPR>(batch, w0, w1, a.H, sub);
+    int pairs[RMAX];
+    const int count = few_take<RMAX>(g.members, pairs);
+    const int chunks = a.H >> 4;
 #pragma unroll
-  for (int r = 0; r < R; r++) {
-    const float xs = a.xs[pairs[r] / a.topk];
-    const float g = (float)lanes_sum<LPR>(acc[0][r]) * (xs * sg) + bg, u = (float)lanes_sum<LPR>(acc[1][r]) * (xs * su) + bu;
-    v[r] = g / (1.0f + expf(-g)) * u;
-  }
-#pragma unroll
-  for (int r = 0; r < R; r++)
-    if (sub == r && r < count && col < a.I) a.act[(int64_t)pairs[r] * a.I + col] = v[r];
-}
-
-// grid: column tiles of 4 waves x pairs (the groups are at most as many).
-template <bool INT8, typename OT, int RMAX, int LPR>
-__global__ __launch_bounds__(256) void few_up_kernel(FewArgs a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = ((int)blockIdx.x * 4 + wave) * (64 / LPR) + lane / LPR;
-  few_groups(a, [&](int group, int expert, unsigned long long members) {
-    if (group != (int)blockIdx.y) return true;
-    while (members) {
-      if (RMAX == 1 || (members & (members - 1)) == 0) few_up_rows<INT8, OT, 1, LPR, 4>(a, expert, members, col, lane % LPR);
-      else few_up_rows<INT8, OT, RMAX, LPR, 2>(a, expert, members, col, lane % LPR);
+    for (int r = 0; r < RMAX; r++) {
+      if (r >= count) break;
+      const v4i* src = (const v4i*)(a.x + (int64_t)(pairs[r] / a.topk) * a.H);
+      for (int c = threadIdx.x; c < chunks; c += 256) *(v4i*)(rows + r * a.H + c * 16) = src[c];
     }
-    return false;
-  });
+    __syncthreads();
+    acc_t acc[2][RMAX] = {};
+    auto fetch = [&](int at, int r) { return *(const v4i*)(rows + (r < count ? r : 0) * a.H + sub * 16 + at); };
+    if (RMAX > 1 && count > 1) {
+      few_dot<INT8, RMAX, LPR, S>(w0, w1, a.H, sub, batch, fetch, acc);
+    } else {
+      acc_t one[2][1] = {};
+      few_dot<INT8, 1, LPR, S>(w0, w1, a.H, sub, batch, fetch, one);
+      acc[0][0] = one[0][0], acc[1][0] = one[1][0];
+    }
+#pragma unroll
+    for (int r = 0; r < RMAX; r++) {
+      if (r >= count) break;
+      const float xs = a.xs[pairs[r] / a.topk];
+      const float gate = (float)lanes_sum<LPR>(acc[0][r]) * (xs * sg) + bg, up = (float)lanes_sum<LPR>(acc[1][r]) * (xs * su) + bu;
+      if (sub == r && col < a.I) a.act[(int64_t)pairs[r] * a.I + col] = gate / (1.0f + expf(-gate)) * up;
+    }
+    if (!g.members) return;
+    __syncthreads();  // the next rows take the place of these
+  }
 }
 
 // Row `pair` of a, quantised into LDS; returns its scale.  Up to 2048 values stay in registers between the maximum and the
 // codes, longer rows are read again.
+constexpr int FEW_KEEP = 8;
+__device__ __forceinline__ void few_act_load(const FewArgs& a, int pair, int lane, v4f (&v)[FEW_KEEP]) {
+  const v4f* src = (const v4f*)(a.act + (int64_t)pair * a.I);
+#pragma unroll
+  for (int k = 0; k < FEW_KEEP; k++) v[k] = src[min(lane + k * 64, (a.I >> 2) - 1)];  // (repeats change no maximum)
+}
 template <bool INT8>
-__device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_t* dst, int lane) {
-  constexpr int KEEP = 8;
+__device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_t* dst, int lane, const v4f (&v)[FEW_KEEP]) {
   const v4f* src = (const v4f*)(a.act + (int64_t)pair * a.I);
   const int chunks = a.I >> 2;
-  v4f v[KEEP];
   uint32_t top = 0;
   auto take = [&](const v4f& c) {
 #pragma unroll
     for (int j = 0; j < 4; j++) top = umax(top, __float_as_uint(c[j]) & 0x7fffffffu);
   };
 #pragma unroll
-  for (int k = 0; k < KEEP; k++) v[k] = lane + k * 64 < chunks ? src[lane + k * 64] : v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < KEEP; k++) take(v[k]);
-  for (int c = lane + KEEP * 64; c < chunks; c += 64) take(src[c]);
+  for (int k = 0; k < FEW_KEEP; k++) take(v[k]);
+  for (int c = lane + FEW_KEEP * 64; c < chunks; c += 64) take(src[c]);
   const float amax0 = __uint_as_float(wave_umax(top));
   float scale, mul;
   if constexpr (INT8) {
@@ -257,74 +304,95 @@ __device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_
     *(uint32_t*)(dst + 4 * c) = row_codes4<INT8 ? ROW_TO_INT8 : ROW_TO_FP8>(f, o);
   };
 #pragma unroll
-  for (int k = 0; k < KEEP; k++)
+  for (int k = 0; k < FEW_KEEP; k++)
     if (lane + k * 64 < chunks) put(lane + k * 64, v[k]);
-  for (int c = lane + KEEP * 64; c < chunks; c += 64) put(c, src[c]);
+  for (int c = lane + FEW_KEEP * 64; c < chunks; c += 64) put(c, src[c]);
   return scale;
 }
 
-template <bool INT8, typename OT, int R, int LPR, int S>
-__device__ __forceinline__ void few_down_rows(const FewArgs& a, int expert, unsigned long long& members, int n0, int sub, int lane, uint8_t* codes,
-                                              float* part) {
-  typedef typename std::conditional<INT8, int, float>::type acc_t;
-  constexpr int COLS = 64 / LPR;
-  const int na = min(n0, a.H - 1), nb = min(n0 + COLS, a.H - 1);
-  const int64_t ra = (int64_t)expert * a.H + na, rb = (int64_t)expert * a.H + nb;
-  const uint8_t* w0 = a.w + ra * a.I + sub * 16;
-  const uint8_t* w1 = a.w + rb * a.I + sub * 16;
-  FewBatch<S> first = {};
-  if (a.I / (LPR * 16) >= S) first = few_load<S, LPR>(w0, w1, 0);
-  int pairs[R];
-  const int count = few_take<R>(members, pairs);
-  float scale[R];
-#pragma unroll
-  for (int r = 0; r < R; r++) scale[r] = r < count ? few_quantise<INT8>(a, pairs[r], codes + r * a.I, lane) : 0.f;
-  // (the rows are this wave's own: its LDS instructions run in order)
-  asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-  const float sa = a.s[ra], sb = a.s[rb];
-  float ba = 0.f, bb = 0.f;
-  if (a.b) {
-    ba = OT::to_f32(((const typename OT::storage*)a.b)[ra]);
-    bb = OT::to_f32(((const typename OT::storage*)a.b)[rb]);
-  }
-  const uint8_t* x = codes + sub * 16;
-  acc_t acc[2][R] = {};
-  few_dot<INT8, R, LPR, S>(w0, w1, a.I, sub, first,
-                           [&](int step, int r) { return *(const v4i*)(x + (r < count ? r : 0) * a.I + step * (LPR * 16)); }, acc);
-  float va[R], vb[R];
-#pragma unroll
-  for (int r = 0; r < R; r++) {
-    const float wt = a.weights[pairs[r]];
-    va[r] = ((float)lanes_sum<LPR>(acc[0][r]) * (scale[r] * sa) + ba) * wt;
-    vb[r] = ((float)lanes_sum<LPR>(acc[1][r]) * (scale[r] * sb) + bb) * wt;
-  }
-#pragma unroll
-  for (int r = 0; r < R; r++)
-    if (sub == r && r < count) {
-      part[pairs[r] * (2 * COLS) + lane / LPR] = va[r];
-      part[pairs[r] * (2 * COLS) + COLS + lane / LPR] = vb[r];
-    }
-  asm volatile("" : : : "memory");  // the next rows overwrite the codes behind these reads
-}
-
-// grid: tiles of 2 * 64 / LPR output columns.  LDS: RMAX rows of I codes for each wave.
+// grid: tiles of 2 * 64 / LPR output columns, a group to a wave in turn.  LDS: RMAX rows of I codes for each wave.
 template <bool INT8, typename OT, int RMAX, int LPR>
 __global__ __launch_bounds__(512) void few_down_kernel(FewArgs a) {
   typedef typename OT::storage OS;
-  constexpr int COLS = 64 / LPR;
+  typedef typename std::conditional<INT8, int, float>::type acc_t;
+  constexpr int COLS = 64 / LPR, S = few_batch(RMAX, LPR);
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ float part[FEW_MAX_PAIRS * 2 * COLS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
+  const int sub = lane % LPR, tile0 = (int)blockIdx.x * 2 * COLS;
+  const int na = min(tile0 + lane / LPR, a.H - 1), nb = min(tile0 + COLS + lane / LPR, a.H - 1);
   uint8_t* codes = smem + wave * RMAX * a.I;
-  const int tile0 = (int)blockIdx.x * 2 * COLS;
-  few_groups(a, [&](int group, int expert, unsigned long long members) {
-    if (group % waves != wave) return true;
-    while (members) {
-      if (RMAX == 1 || (members & (members - 1)) == 0) few_down_rows<INT8, OT, 1, LPR, 4>(a, expert, members, tile0 + lane / LPR, lane % LPR, lane, codes, part);
-      else few_down_rows<INT8, OT, RMAX, LPR, 2>(a, expert, members, tile0 + lane / LPR, lane % LPR, lane, codes, part);
+  const int mine = few_expert(a, lane);
+  unsigned long long rest = __ballot(mine >= 0);
+  int turn = wave;
+  auto next = [&](const FewGroup& g) -> FewGroup {
+    if (g.members) return g;  // more rows of this group than one pass serves
+    while (rest) {
+      const int expert = __builtin_amdgcn_readlane(mine, __builtin_ctzll(rest));
+      const unsigned long long members = __ballot(mine == expert);
+      rest &= ~members;
+      if (turn-- == 0) {
+        turn = waves - 1;
+        return {expert, members};
+      }
     }
-    return true;
-  });
+    return {0, 0};
+  };
+  // A group's first row, then its first weights: loads return in the order of their requests.
+  v4f row[FEW_KEEP];
+  FewBatch<S> batch;
+  const uint8_t *w0, *w1;
+  auto request = [&](const FewGroup& g) {
+    few_act_load(a, __builtin_ctzll(g.members), lane, row);
+    w0 = a.w + ((int64_t)g.expert * a.H + na) * a.I + sub * 16;
+    w1 = a.w + ((int64_t)g.expert * a.H + nb) * a.I + sub * 16;
+    few_load_first<S, LPR>(batch, w0, w1, a.I, sub);
+  };
+  FewGroup g = next({0, 0});
+  if (g.members) request(g);
+  while (g.members) {
+    int pairs[RMAX];
+    const int count = few_take<RMAX>(g.members, pairs);
+    float scale[RMAX];
+#pragma unroll
+    for (int r = 0; r < RMAX; r++) {
+      scale[r] = 0.f;
+      if (r >= count) continue;
+      if (r > 0) few_act_load(a, pairs[r], lane, row);
+      scale[r] = few_quantise<INT8>(a, pairs[r], codes + r * a.I, lane, row);
+    }
+    // (the rows are this wave's own: its LDS instructions run in order)
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    const int64_t ra = (int64_t)g.expert * a.H + na, rb = (int64_t)g.expert * a.H + nb;
+    const float sa = a.s[ra], sb = a.s[rb];
+    float ba = 0.f, bb = 0.f;
+    if (a.b) {
+      ba = OT::to_f32(((const OS*)a.b)[ra]);
+      bb = OT::to_f32(((const OS*)a.b)[rb]);
+    }
+    acc_t acc[2][RMAX] = {};
+    auto fetch = [&](int at, int r) { return *(const v4i*)(codes + (r < count ? r : 0) * a.I + sub * 16 + at); };
+    if (RMAX > 1 && count > 1) {
+      few_dot<INT8, RMAX, LPR, S>(w0, w1, a.I, sub, batch, fetch, acc);
+    } else {
+      acc_t one[2][1] = {};
+      few_dot<INT8, 1, LPR, S>(w0, w1, a.I, sub, batch, fetch, one);
+      acc[0][0] = one[0][0], acc[1][0] = one[1][0];
+    }
+    asm volatile("" : : : "memory");  // the next rows overwrite the codes behind these reads
+#pragma unroll
+    for (int r = 0; r < RMAX; r++) {
+      if (r >= count) break;
+      const float wt = a.weights[pairs[r]];
+      const float va = ((float)lanes_sum<LPR>(acc[0][r]) * (scale[r] * sa) + ba) * wt, vb = ((float)lanes_sum<LPR>(acc[1][r]) * (scale[r] * sb) + bb) * wt;
+      if (sub == r) {
+        part[pairs[r] * (2 * COLS) + lane / LPR] = va;
+        part[pairs[r] * (2 * COLS) + COLS + lane / LPR] = vb;
+      }
+    }
+    g = next(g);
+    if (g.members) request(g);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < a.M * 2 * COLS; i += blockDim.x) {
     const int t = i / (2 * COLS), c = i % (2 * COLS);
@@ -338,24 +406,24 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs a) {
   }
 }
 
-// Lanes per weight row: the fewest (8, the most work for a wave) that still give every CU `want` waves.
-static int few_lanes(int64_t rows_of_groups, int rows_at_8, int want) {
-  for (int lpr = 8; lpr < 32; lpr *= 2)
-    if (rows_of_groups * lpr >= (int64_t)want * device_cus() * rows_at_8 * 8) return lpr;
-  return 32;
-}
-
 template <bool INT8, typename OT, int RMAX, int LPR>
 static int few_start_up(const FewArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)ceil_div(a.I, 4 * (64 / LPR)), (unsigned)(a.M * a.topk));
-  hipLaunchKernelGGL((few_up_kernel<INT8, OT, RMAX, LPR>), grid, dim3(256), 0, st, a);
+  auto kern = few_up_kernel<INT8, OT, RMAX, LPR>;
+  const int smem = std::min(RMAX, a.M * a.topk) * a.H;
+  if (smem > 56 * 1024) {
+    static SmemAttrOnce attr;
+    const hipError_t e = raise_dynamic_smem(attr, (const void*)kern, smem);
+    if (e != hipSuccess) return fail(SGLAMD_EHIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kern, grid, dim3(256), smem, st, a);
   return check_launch("few_up");
 }
 template <bool INT8, typename OT, int RMAX, int LPR>
-static int few_start_down(const FewArgs& a, int waves, hipStream_t st) {
+static int few_start_down(const FewArgs& a, hipStream_t st) {
   auto kern = few_down_kernel<INT8, OT, RMAX, LPR>;
-  const int smem = waves * RMAX * a.I;
-  if (smem > 60 * 1024) {
+  const int waves = std::min(a.M * a.topk, FEW_DOWN_WAVES), smem = waves * RMAX * a.I;
+  if (smem > 56 * 1024) {
     static SmemAttrOnce attr;
     const hipError_t e = raise_dynamic_smem(attr, (const void*)kern, smem);
     if (e != hipSuccess) return fail(SGLAMD_EHIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
@@ -366,21 +434,24 @@ static int few_start_down(const FewArgs& a, int waves, hipStream_t st) {
 
 template <bool INT8, typename OT>
 static int few_layer(const FewArgs& up, const FewArgs& down, hipStream_t st) {
-  const int pairs = up.M * up.topk;
-  const int waves = pairs < 8 ? pairs : 8;
-  // Rows that one pass over an expert's weights may serve: as many as there are tokens, as LDS holds of them.
+  const int pairs = up.M * up.topk, cus = device_cus();
+  // Rows that one pass over an expert's weights serves: as many as there are tokens, as LDS holds of them.
   int rmax = up.M == 1 ? 1 : up.M == 2 ? 2 : 4;
-  while (rmax > 1 && waves * rmax * up.I > 64 * 1024) rmax /= 2;
-  const int lpr1 = few_lanes((int64_t)up.I * pairs, 8, 12), lpr2 = few_lanes((int64_t)up.H * pairs, 16, 12);
-#define SGLAMD_FEW(START, R, LPR, ...) (LPR == 8 ? START<INT8, OT, R, 8>(__VA_ARGS__) : LPR == 16 ? START<INT8, OT, R, 16>(__VA_ARGS__) : START<INT8, OT, R, 32>(__VA_ARGS__))
-  const int rc = rmax == 1   ? SGLAMD_FEW(few_start_up, 1, lpr1, up, st)
-                 : rmax == 2 ? SGLAMD_FEW(few_start_up, 2, lpr1, up, st)
-                             : SGLAMD_FEW(few_start_up, 4, lpr1, up, st);
+  while (rmax > 1 && (std::min(pairs, FEW_DOWN_WAVES) * rmax * up.I > FEW_LDS || rmax * up.H > FEW_LDS)) rmax /= 2;
+  // Lanes per weight row.  First launch: eight, where that gives a CU six waves, else 32 (8 | 32 lanes: 7168 x 2048, one token, eight waves
+  // a CU, 37.6 | 38.5 us; 2048 x 768, three tokens, nine, 15.0 | 16.7; 4096 x 1536, one token, 4.5, 16.5 | 14.9; 2048 x 768, one token,
+  // three, 8.5 | 6.8).  Second: the fewest of 8, 16 and 32 whose column tiles reach every CU (8 | 16: 4096 columns, 256 tiles of 8,
+  // 10.2 | 12.0; 2048 columns, 128 tiles of 8, 17.4 | 13.9; 8 | 16 | 32: 1024 columns 9.2 | 8.2 | 7.8).
+  const bool wide = (int64_t)pairs * up.I >= 6 * 8 * (int64_t)cus;
+  const int lpr = up.H >= 16 * cus ? 8 : up.H >= 8 * cus ? 16 : 32;
+#define SGLAMD_FEW_UP(R) (wide ? few_start_up<INT8, OT, R, 8>(up, st) : few_start_up<INT8, OT, R, 32>(up, st))
+#define SGLAMD_FEW_DOWN(R) \
+  (lpr == 8 ? few_start_down<INT8, OT, R, 8>(down, st) : lpr == 16 ? few_start_down<INT8, OT, R, 16>(down, st) : few_start_down<INT8, OT, R, 32>(down, st))
+  const int rc = rmax == 1 ? SGLAMD_FEW_UP(1) : rmax == 2 ? SGLAMD_FEW_UP(2) : SGLAMD_FEW_UP(4);
   if (rc) return rc;
-  return rmax == 1   ? SGLAMD_FEW(few_start_down, 1, lpr2, down, waves, st)
-         : rmax == 2 ? SGLAMD_FEW(few_start_down, 2, lpr2, down, waves, st)
-                     : SGLAMD_FEW(few_start_down, 4, lpr2, down, waves, st);
-#undef SGLAMD_FEW
+  return rmax == 1 ? SGLAMD_FEW_DOWN(1) : rmax == 2 ? SGLAMD_FEW_DOWN(2) : SGLAMD_FEW_DOWN(4);
+#undef SGLAMD_FEW_UP
+#undef SGLAMD_FEW_DOWN
 }
 
 }  // namespace sglamd
@@ -407,10 +478,8 @@ extern "C" int sglamd_fused_experts_few_tokens(const void* x, const float* x_sca
                  "%s: %lld tokens of %d experts are more than %d pairs", op, (long long)M, topk, FEW_MAX_PAIRS);
   SGLAMD_REQUIRE(H > 0 && I > 0 && H % 16 == 0 && I % 16 == 0, SGLAMD_EINVAL,
                  "%s: hidden (%lld) and intermediate (%lld) sizes must be multiples of 16", op, (long long)H, (long long)I);
-  SGLAMD_REQUIRE(H < (1ll << 24) && I <= FEW_MAX_INTER, SGLAMD_ENOTSUP, "%s: sizes %lld and %lld are beyond %d and %d", op, (long long)H,
-                 (long long)I, (1 << 24) - 1, FEW_MAX_INTER);
-  // (sums of 2^31 / 128^2 int8 products stay inside 32 bits)
-  SGLAMD_REQUIRE(q_dtype != SGLAMD_I8 || H <= 131071, SGLAMD_ENOTSUP, "%s: int8 rows of %lld are beyond 131071", op, (long long)H);
+  SGLAMD_REQUIRE(H <= FEW_MAX_HIDDEN && I <= FEW_MAX_INTER, SGLAMD_ENOTSUP, "%s: sizes %lld and %lld are beyond %d and %d", op, (long long)H,
+                 (long long)I, FEW_MAX_HIDDEN, FEW_MAX_INTER);
   SGLAMD_REQUIRE((((uintptr_t)x | (uintptr_t)w13 | (uintptr_t)w2 | (uintptr_t)workspace) & 15) == 0, SGLAMD_EINVAL,
                  "%s: rows, weights and workspace must be 16-byte aligned", op);
   SGLAMD_REQUIRE(workspace_bytes >= M * topk * I * 4, SGLAMD_EINVAL, "%s: workspace too small", op);

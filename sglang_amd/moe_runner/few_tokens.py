@@ -36,7 +36,7 @@ def fused_experts_few_tokens(
     token), w1 [E, 2 * I, H] and w2 [E, H, I] of that dtype, w1_scale / w2_scale one float32 per output channel, b1 / b2 one
     value per output channel in out_dtype, topk_weights and topk_ids [M, topk].  Pairs whose id is outside [0, E) contribute
     nothing.  Between the products the rows stay in float32 and are quantised per (token, expert) pair by the formulas of
-    fused_row_quant; the output is rounded once.  H, I multiples of 16, I <= 16384; more than MAX_PAIRS pairs raise
+    fused_row_quant; the output is rounded once.  H, I multiples of 16, H <= 32768, I <= 16384; more than MAX_PAIRS pairs raise
     NotImplementedError (fused_experts takes them)."""
     return _C.experts_few_tokens(hidden_q, hidden_scale, w1, w2, w1_scale, w2_scale, topk_weights, topk_ids, out_dtype, b1, b2,
                                  1.0 if routed_scaling_factor is None else routed_scaling_factor)

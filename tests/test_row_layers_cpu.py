@@ -70,7 +70,7 @@ def test_few_tokens_refuses():
     good = [64, 64, 4, 2, 256, 128, 8, 2, 64, 64, None, 64, 64, None, 64, 64, 5, 64, 2, 1.0, 64, 1 << 20, None]
     for at, value, code in ((0, None, -1), (1, None, -1), (8, None, -1), (9, None, -1), (11, None, -1), (12, None, -1), (14, None, -1), (15, None, -1),
                             (17, None, -1), (20, None, -1), (2, 2, -1), (18, 0, -1), (16, 2, -1), (3, 0, -1), (6, 0, -1), (7, 0, -1), (3, 33, -2),
-                            (7, 65, -2), (4, 264, -1), (5, 120, -1), (5, 16400, -2), (4, 131088, -2), (0, 72, -1), (20, 72, -1), (21, 1000, -1),
+                            (7, 65, -2), (4, 264, -1), (5, 120, -1), (5, 16400, -2), (4, 32784, -2), (0, 72, -1), (20, 72, -1), (21, 1000, -1),
                             (4, 1 << 24, -2), (3, 1 << 40, -2)):
         args = list(good)
         args[at] = value
