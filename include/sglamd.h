@@ -231,6 +231,17 @@ int sglamd_int8_scaled_mm_azp(const void* a, int64_t lda, const void* b, int64_t
                               int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                               void* stream);
 
+/* The linear layer on an int8 weight with a scale per output channel, from one call: x [M, K] (F16/BF16, rows x_row_stride
+ * elements apart) quantised per token, then the product in dtype.  Without weight_sums the arithmetic of
+ * sglamd_per_token_quant_int8 and sglamd_int8_scaled_mm (contiguous 16-byte aligned rows), with them that of
+ * sglamd_per_token_quant_int8_asym and sglamd_int8_scaled_mm_azp; the same bits either way, in one launch where a few short rows are
+ * quantised by the product's own workgroups (M <= 16, K % 128 == 0).  q int8 [M, K], sa fp32 [M] and zp int32 [M] (NULL without
+ * weight_sums) are scratch; workspace as for the products. */
+int sglamd_int8_row_linear(const void* x, int64_t x_row_stride, int dtype, int64_t M, int64_t K, const void* w,
+                           int64_t ldb, const float* sb, const int32_t* weight_sums, const void* bias, void* out,
+                           int64_t ldc, int64_t N, void* q, float* sa, int32_t* zp, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 /* sums[n] = sum over k of b[n, k], b int8 [N, K] with rows of ldb bytes, any K below 2^24 and any alignment. */
 int sglamd_int8_weight_sums(const void* b, int64_t ldb, int64_t N, int64_t K, int32_t* sums, void* stream);
 

@@ -37,6 +37,7 @@ SIGNATURES = {
     "sglamd_fp8_scaled_mm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
     "sglamd_int8_scaled_mm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
     "sglamd_int8_scaled_mm_azp": [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i, _i64, _i64, _i64, _p, _i64, _p],
+    "sglamd_int8_row_linear": [_p, _i64, _i, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _i64, _p],
     "sglamd_int8_weight_sums": [_p, _i64, _i64, _i64, _p, _p],
     "sglamd_gemm_workspace_bytes": [_i64, _i64, _i64],
     "sglamd_last_gemm_kernel": [],

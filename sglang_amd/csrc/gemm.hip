@@ -16,6 +16,8 @@ extern template int dispatch_quantising<GEMM_ROW_FP8, false>(const GemmArgs&, in
 extern template int dispatch_out<GEMM_ROW_FP8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 extern template int dispatch_out<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 extern template int dispatch_out_zero_point<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
+extern template int dispatch_quantising<GEMM_ROW_INT8, false>(const GemmArgs&, int, hipStream_t, bool);
+extern template int dispatch_quantising_zero_point<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, bool);
 extern template int dispatch_out<GEMM_BLOCK_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
 
 static int check_common(const char* op, const void* a, const void* b, const void* c, int64_t M, int64_t N, int64_t K,
@@ -261,6 +263,48 @@ extern "C" int sglamd_int8_scaled_mm_azp(const void* a, int64_t lda, const void*
   SGLAMD_REQUIRE(K <= 65536, SGLAMD_ENOTSUP, "%s: K (%lld) is beyond 65536", op, (long long)K);
   return rowwise(GEMM_ROW_INT8, op, a, lda, b, ldb, sa, sb, bias, out, ldc, out_dtype, M, N, K, workspace, workspace_bytes, stream, zp,
                  weight_sums);
+}
+
+extern "C" int sglamd_int8_row_linear(const void* x, int64_t x_row_stride, int dtype, int64_t M, int64_t K, const void* w, int64_t ldb,
+                                      const float* sb, const int32_t* weight_sums, const void* bias, void* out, int64_t ldc, int64_t N,
+                                      void* q, float* sa, int32_t* zp, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* op = "int8_row_linear";
+  SGLAMD_REQUIRE(x && w && sb && out && q && sa && (zp || !weight_sums), SGLAMD_EINVAL, "%s: null pointer", op);
+  SGLAMD_REQUIRE(dtype == SGLAMD_BF16 || dtype == SGLAMD_F16, SGLAMD_EINVAL, "%s: dtype must be Half or BFloat16", op);
+  SGLAMD_REQUIRE(x_row_stride >= K, SGLAMD_EINVAL, "%s: row stride smaller than the row", op);
+  SGLAMD_REQUIRE(!weight_sums || K <= 65536, SGLAMD_ENOTSUP, "%s: K (%lld) is beyond 65536", op, (long long)K);
+  const DeviceScope scope;
+  int rc = check_common(op, q, w, out, M, N, K, K, ldb, ldc);
+  if (rc) return rc;
+  if (M == 0) return SGLAMD_OK;
+  if (linear_quantises(M, K, true) && K % 128 == 0 && ((uintptr_t)x % 16) == 0 && x_row_stride % 8 == 0 && M * x_row_stride * 2 < 0x7ffffff0ll) {
+    GemmArgs g = {};
+    g.A16 = x;
+    g.lda16 = x_row_stride * 2;
+    g.act_mode = 1;
+    g.lda = K;
+    g.B = (const uint8_t*)w;
+    g.ldb = ldb;
+    g.sb = sb;
+    g.route_ids = weight_sums;
+    g.bias = bias;
+    g.C = out;
+    g.ldc = ldc;
+    g.M = (int)M;
+    g.N = (int)N;
+    g.K = (int)K;
+    const auto run = weight_sums ? dispatch_quantising_zero_point<GEMM_ROW_INT8> : dispatch_quantising<GEMM_ROW_INT8, false>;
+    if (gemm8_skinny_ok(g, M) && run(g, dtype, (hipStream_t)stream, false)) return run(g, dtype, (hipStream_t)stream, true);
+  }
+  if (weight_sums) {
+    rc = sglamd_per_token_quant_int8_asym(x, x_row_stride, dtype, M, K, (int8_t*)q, sa, zp, stream);
+  } else {
+    SGLAMD_REQUIRE(M == 1 || x_row_stride == K, SGLAMD_ENOTSUP, "%s: rows without zero points must be contiguous", op);
+    rc = sglamd_per_token_quant_int8(x, dtype, (int8_t*)q, sa, M, K, stream);
+  }
+  if (rc) return rc;
+  return rowwise(GEMM_ROW_INT8, op, q, K, w, ldb, sa, sb, bias, out, ldc, dtype, M, N, K, workspace, workspace_bytes, stream,
+                 weight_sums ? zp : nullptr, weight_sums);
 }
 
 extern "C" int sglamd_last_gemm_kernel(void) { return last_kernel; }

@@ -271,7 +271,7 @@ static int dispatch_dense(const GemmArgs& g, hipStream_t st, void* workspace, in
   return gemm8_launch<128, 128, 2, 2, MODE, OT, false>(g, st);
 }
 
-// An FP8 linear layer of a few rows in one launch (gemm8_skinny_quantising).
+// A linear layer of a few rows in one launch (gemm8_skinny_quantising).
 template <int MODE, bool BIASED>
 int dispatch_quantising(const GemmArgs& g, int out_dtype, hipStream_t st, bool launch) {
   if (launch) {
@@ -282,6 +282,17 @@ int dispatch_quantising(const GemmArgs& g, int out_dtype, hipStream_t st, bool l
     return out_dtype == SGLAMD_BF16 ? gemm8_skinny_quantising<MODE, Biased<BF16>>(g, st, launch)
                                     : gemm8_skinny_quantising<MODE, Biased<F16>>(g, st, launch);
   return out_dtype == SGLAMD_BF16 ? gemm8_skinny_quantising<MODE, BF16>(g, st, launch) : gemm8_skinny_quantising<MODE, F16>(g, st, launch);
+}
+
+// The same for int8 rows with zero points.
+template <int MODE>
+int dispatch_quantising_zero_point(const GemmArgs& g, int out_dtype, hipStream_t st, bool launch) {
+  if (launch) {
+    RAN(SGLAMD_KERNEL_STREAMING);
+    strip_last_shape = 0;
+  }
+  return out_dtype == SGLAMD_BF16 ? gemm8_skinny_quantising<MODE, ZeroPoint<BF16>>(g, st, launch)
+                                  : gemm8_skinny_quantising<MODE, ZeroPoint<F16>>(g, st, launch);
 }
 
 template <int MODE>

@@ -3,4 +3,5 @@
 
 namespace sglamd {
 template int dispatch_out<GEMM_ROW_INT8>(const GemmArgs&, int, hipStream_t, void*, int64_t);
+template int dispatch_quantising<GEMM_ROW_INT8, false>(const GemmArgs&, int, hipStream_t, bool);
 }  // namespace sglamd

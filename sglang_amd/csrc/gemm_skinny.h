@@ -20,7 +20,7 @@
 //     block scale; the KW partial sums meet in LDS and leave as 8-byte stores.
 // The same kernel walks the fused-MoE sorted-block schedule (MOE = true): tile rows are gathered
 // through sorted_token_ids, the expert comes from expert_ids.
-// With AQ > 0 (block FP8) the activations are not read as FP8 at all: the kernel takes the 16-bit source rows and quantises
+// With AQ > 0 (block FP8; DQ: the row modes too) the activations are not read as FP8 at all: the kernel takes the 16-bit source rows and quantises
 // the tile's few rows per 128-wide group into LDS while its first weight blocks are on their way, with the very arithmetic
 // of the stand-alone group-quant kernel, so a decode-sized layer saves that kernel's launch.
 //   MoE, AQ = 4: at most four real rows per sorted block, found through the sorted list and loaded into registers.
@@ -36,7 +36,7 @@
 #include <stdlib.h>
 
 #include "gemm_core.h"
-#include "quant_core.h"
+#include "row_out.h"
 
 namespace sglamd {
 
@@ -132,8 +132,9 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
   constexpr int LOADS = AQ > 0 ? 2 * FN + (BLK ? 1 : 0) : 2 * FN + 2 * FM + (BLK ? 2 : 0);
   constexpr bool DQ = AQ > 0 && !MOE;
   constexpr bool SOLO = AQ == 1 && MOE;  // the routed pairs of one token: sorted block p is pair p
-  static_assert(AQ == 0 || ((MODE == GEMM_BLOCK_FP8 || (MODE == GEMM_ROW_FP8 && !MOE)) && FM == 1 && AQ <= 16),
-                "in-kernel activation quantisation: FP8, one row tile");
+  static_assert(AQ == 0 || ((MODE == GEMM_BLOCK_FP8 || (!BLK && !MOE)) && FM == 1 && AQ <= 16),
+                "in-kernel activation quantisation: FP8, or the row modes of a dense launch, one row tile");
+  constexpr bool ASYM = DQ && out_zero_point<OT>;
   static_assert(PD >= 1 && PD * LOADS < 64, "the vmcnt field counts up to 63 loads in flight");
   // a wave's partial tiles wait for the cross-wave sum in its last ring slot when they fit there; wide tiles put
   // them side by side over the whole ring area instead (behind a barrier: every wave's loads have landed by then)
@@ -146,6 +147,8 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
   // for the cross-wave sum at the end of a tile.
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   __shared__ uint32_t s_amax[DQ && !BLK ? 16 : 1];  // DQ, row scales: the rows' maxima (bits of floats that are not negative)
+  __shared__ uint32_t s_low[ASYM ? 16 : 1];         // with zero points: of the negated values
+  __shared__ int s_zp[ASYM ? 16 : 1];
   __shared__ int s_rows[2][FM * 16];  // MoE: sorted slot ids of the tile's rows, for the current and the next tile
 
   const int tid = threadIdx.x;
@@ -542,18 +545,36 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
               const int gi = (p0 + p) * 8 * QW + (tid >> 3);
               XS e[16];
               __builtin_memcpy(e, raw[p], 32);
-              float m = 0.f;
+              if constexpr (ASYM) {
+                RowStats t = {0.f, 0u, 0u};
+                float poison = 0.f;
 #pragma unroll
-              for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(OT::to_f32(e[i])));
-              m = lanes_max<8>(m);
-              if ((lane & 7) == 0 && gi < dq_groups) atomicMax(&s_amax[gi / nkb], __float_as_uint(m));
+                for (int i = 0; i < 16; i++) {
+                  const float v = OT::to_f32(e[i]);
+                  row_stats_add<ROW_PLAIN, ROW_TO_ASYM>(t, v);
+                  poison = fmaf(v, 0.f, poison);
+                }
+                row_stats_poison(t, poison);
+                t.hi = lanes8_umax(t.hi & 0x7fffffffu);
+                t.lo = lanes8_umax(t.lo & 0x7fffffffu);
+                if ((lane & 7) == 0 && gi < dq_groups) {
+                  atomicMax(&s_amax[gi / nkb], t.hi);
+                  atomicMax(&s_low[gi / nkb], t.lo);
+                }
+              } else {
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) m = fmaxf(m, fabsf(OT::to_f32(e[i])));
+                m = lanes_max<8>(m);
+                if ((lane & 7) == 0 && gi < dq_groups) atomicMax(&s_amax[gi / nkb], __float_as_uint(m));
+              }
             }
           asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
         }
 #pragma unroll
         for (int p = 0; p < SKINNY_DQ_PASSES; p++)
           if (p0 + p < dq_passes) {
-            // group_quant_body's arithmetic (reciprocal form, float scales); row scales: row_quant_body's
+            // group_quant_body's arithmetic (reciprocal form, float scales); row scales: row_quant_body's, with zero points row_out.h's
             const int gi = (p0 + p) * 8 * QW + (tid >> 3);
             XS e[16];
             float x[16];
@@ -564,10 +585,19 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
               x[i] = OT::to_f32(e[i]);
               if (BLK) amax = fmaxf(amax, fabsf(x[i]));
             }
-            float mul;
+            float mul = 0.f;
+            RowScale asym = {};
             if constexpr (BLK) {
               amax = lanes_max<8>(amax);
               mul = g.q_max / amax;
+            } else if constexpr (ASYM) {
+              const int r = gi < dq_groups ? gi / nkb : 0;
+              asym = row_scale<ROW_PLAIN, ROW_TO_ASYM>(RowOutArgs{}, RowStats{0.f, s_amax[r], s_low[r]});
+              amax = asym.scale;
+            } else if constexpr (MODE == GEMM_ROW_INT8) {
+              const float top = fmaxf(__uint_as_float(s_amax[gi < dq_groups ? gi / nkb : 0]), 1e-10f);
+              mul = 127.0f / top;
+              amax = top / 127.0f;
             } else {
               const float scale = __uint_as_float(s_amax[gi < dq_groups ? gi / nkb : 0]) / 448.0f;
               mul = (scale == 0.f) ? 0.f : 1.0f / scale;
@@ -575,16 +605,27 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
             }
             uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              o[i] = pack4_e4m3(clampf(x[4 * i] * mul, g.q_min, g.q_max), clampf(x[4 * i + 1] * mul, g.q_min, g.q_max),
-                                clampf(x[4 * i + 2] * mul, g.q_min, g.q_max), clampf(x[4 * i + 3] * mul, g.q_min, g.q_max));
+            for (int i = 0; i < 4; i++) {
+              if constexpr (ASYM) {
+                o[i] = row_codes4<ROW_TO_ASYM>(x + 4 * i, asym);
+              } else if constexpr (MODE == GEMM_ROW_INT8) {
+                o[i] = pack4_low(round_away(x[4 * i] * mul), round_away(x[4 * i + 1] * mul), round_away(x[4 * i + 2] * mul),
+                                 round_away(x[4 * i + 3] * mul));
+              } else {
+                o[i] = pack4_e4m3(clampf(x[4 * i] * mul, g.q_min, g.q_max), clampf(x[4 * i + 1] * mul, g.q_min, g.q_max),
+                                  clampf(x[4 * i + 2] * mul, g.q_min, g.q_max), clampf(x[4 * i + 3] * mul, g.q_min, g.q_max));
+              }
+            }
             if (gi < dq_groups) {
               const int r = SOLO ? 0 : gi / nkb, c = gi - r * nkb;
               *(v4i*)(xq_rows + r * xq_stride + c * 128 + (lane & 7) * 16) = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
               if constexpr (BLK) {
                 if ((lane & 7) == 0) xq_scales[r * nkb + c] = amax * (1.0f / g.q_max);
               } else {
-                if ((lane & 7) == 0 && c == 0) xq_scales[r] = amax;
+                if ((lane & 7) == 0 && c == 0) {
+                  xq_scales[r] = amax;
+                  if (ASYM) s_zp[r] = (int)asym.zp;
+                }
               }
             }
           }
@@ -600,6 +641,7 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
   int tile = blockIdx.x;
   if (!tile_exists(tile)) return;
   fetch_rows(tile / tiles_n);
+  if (ASYM && tid < 16) s_low[tid] = 0;
   if (DQ && !BLK && tid < 16) s_amax[tid] = 0;  // (visible behind the barrier in front of the first maxima)
   if (SOLO && g.sum_tiles > 0 && !g.sum_out)
     for (int i = blockIdx.x * (64 * KW) + tid; i < g.sum_tiles; i += gridDim.x * (64 * KW)) g.sum_count[i] = 0;
@@ -757,7 +799,8 @@ __global__ __launch_bounds__(64 * QW) void gemm8_skinny_kernel(GemmArgs g) {
       const float* sb_row = g.sb;
       const OS* bias = (const OS*)g.bias;
       int minus_zp = 0;
-      if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[out_row];
+      if constexpr (ASYM) minus_zp = -s_zp[out_row];
+      else if constexpr (out_zero_point<OT>) minus_zp = -((const int32_t*)g.A16)[out_row];
       if constexpr (!gemm_is_block(MODE)) {
         if constexpr (DQ) sam = xq_scales[out_row];
         else sam = g.sa[MOE ? (out_row / g.top_k) * g.sa_sm : out_row];

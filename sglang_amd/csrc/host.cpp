@@ -716,19 +716,11 @@ Tensor int8_linear(const Tensor& x, const Tensor& weight, const Tensor& ws, cons
   const int64_t q = sc.take(m * k), sa = sc.take(4 * m), zp = sums ? sc.take(4 * m) : 0;
   const int64_t wb = sglamd_gemm_workspace_bytes(m, n, k), wp = sc.take(wb > 0 ? wb : 0);
   sc.allocate(x);
-  void* st = stream_of(x);
-  void* wsp = wb > 0 ? sc.at(wp) : nullptr;
-  if (sums) {
-    check(sglamd_per_token_quant_int8_asym(x.data_ptr(), ld(x, 0), tag(t), m, k, (int8_t*)sc.at(q), (float*)sc.at(sa), (int32_t*)sc.at(zp), st));
-    check(sglamd_int8_scaled_mm_azp(sc.at(q), k, weight.data_ptr(), ld(weight, 1), (float*)sc.at(sa), ws.data_ptr<float>(),
-                                    (int32_t*)sc.at(zp), sums->data_ptr<int32_t>(), bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, tag(t),
-                                    m, n, k, wsp, wb, st));
-    return out;
-  }
-  const Tensor rows = x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
-  check(sglamd_per_token_quant_int8(rows.data_ptr(), tag(t), (int8_t*)sc.at(q), (float*)sc.at(sa), m, k, st));
-  check(sglamd_int8_scaled_mm(sc.at(q), k, weight.data_ptr(), ld(weight, 1), (float*)sc.at(sa), ws.data_ptr<float>(),
-                              bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, tag(t), m, n, k, wsp, wb, st));
+  // (rows without zero points are quantised from contiguous, 16-byte aligned ones)
+  const Tensor rows = sums || (x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0) ? x : x.clone(at::MemoryFormat::Contiguous);
+  check(sglamd_int8_row_linear(rows.data_ptr(), ld(rows, 0), tag(t), m, k, weight.data_ptr(), ld(weight, 1), ws.data_ptr<float>(),
+                               sums ? sums->data_ptr<int32_t>() : nullptr, bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, n, sc.at(q),
+                               (float*)sc.at(sa), sums ? (int32_t*)sc.at(zp) : nullptr, wb > 0 ? sc.at(wp) : nullptr, wb, stream_of(x)));
   return out;
 }
 

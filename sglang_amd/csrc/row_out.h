@@ -58,12 +58,14 @@ __device__ __forceinline__ float lanes16_sum(float v) {
   return v;
 }
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t lanes16_umax(uint32_t v) {
+__device__ __forceinline__ uint32_t lanes8_umax(uint32_t v) {
   v = umax(v, dpp_u<0xB1>(v));
   v = umax(v, dpp_u<0x4E>(v));
-  v = umax(v, dpp_u<0x141>(v));
-  v = umax(v, dpp_u<0x140>(v));
-  return v;
+  return umax(v, dpp_u<0x141>(v));
+}
+__device__ __forceinline__ uint32_t lanes16_umax(uint32_t v) {
+  v = lanes8_umax(v);
+  return umax(v, dpp_u<0x140>(v));
 }
 __device__ __forceinline__ float wave_sum(float v) {
   const int x = __float_as_int(lanes16_sum(v));

@@ -130,6 +130,49 @@ def test_linear(dev, m, n, k, dtype, asym, with_bias):
     assert torch.equal(apply_int8_linear(x.view(1, m, k), w.t(), sb, weight_sums=sums, bias=bias), out.view(1, m, n))
 
 
+@pytest.mark.parametrize("n,k", [(64, 128), (1024, 256), (7168, 16384), (2112, 7168), (24576, 1536), (576, 4096), (36864, 640), (4160, 2432), (264, 2064)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 12, 16])
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("dtype,with_bias", [(torch.bfloat16, False), (torch.float16, True)])
+def test_linear_of_a_few_rows_quantised_in_the_product(dev, m, n, k, asym, dtype, with_bias):
+    """The row's extremes span all of its pieces, several waves and passes; rows on one side of zero, of zeros, with a NaN or an
+    infinity; a view into longer rows."""
+    from sglang_amd import int8_scaled_mm, int8_scaled_mm_azp
+    from sglang_amd.quantization.int8_kernel import per_token_quant_int8, per_token_quant_int8_asym
+    from sglang_amd.quantization.int8_utils import apply_int8_linear, int8_weight_sums
+
+    g = torch.Generator(device=dev).manual_seed(m + n + k)
+    w = torch.randint(-128, 128, (n, k), generator=g, device=dev, dtype=torch.int8)
+    ws = torch.rand(n, 1, generator=g, device=dev) * 1e-4 + 1e-5
+    b = torch.randn(n, generator=g, device=dev).to(dtype) if with_bias else None
+    sums = int8_weight_sums(w.t()) if asym else None
+    for kind in ("plain", "zeros", "one side", "nan", "inf", "view"):
+        x = torch.randn(m, k + (64 if kind == "view" else 0), generator=g, device=dev).to(dtype)
+        x[-1, k - 1] = 50.0  # the extreme of a row in its last piece
+        if kind == "zeros":
+            x[0] = 0
+        elif kind == "one side":
+            x = -x.abs() - 1
+        elif kind == "nan":
+            x[m // 2, k // 2] = float("nan")
+        elif kind == "inf":
+            x[m // 2, 3] = float("-inf")
+        elif kind == "view":
+            x = x[:, :k]
+        print(f"one launch, int8, M={m} N={n} K={k} {dtype} {kind}", flush=True)
+        out = apply_int8_linear(x, w.t(), ws, sums, bias=b)
+        if asym:
+            q, s, zp = per_token_quant_int8_asym(x)
+            ref = int8_scaled_mm_azp(q, w.t(), s, ws, dtype, zp, sums, b)
+        else:
+            q, s = per_token_quant_int8(x.contiguous())
+            ref = int8_scaled_mm(q, w.t(), s, ws, dtype, b)
+        assert torch.equal(out.isnan(), ref.isnan())
+        assert torch.equal(out.nan_to_num(), ref.nan_to_num())
+        if asym and kind in ("nan", "inf"):
+            assert out[m // 2].isnan().all() and out.isnan().any(dim=1).sum() == 1
+
+
 def test_linear_of_views_one_scale_and_no_rows(dev):
     from sglang_amd.quantization.int8_utils import apply_int8_linear, int8_weight_sums
 

@@ -63,6 +63,21 @@ def test_asymmetric_product_refuses():
     assert f(*[0 if i == 12 else v for i, v in enumerate(good)]) == 0
 
 
+def test_int8_linear_refuses():
+    f = _lib().sglamd_int8_row_linear
+    # x, x_stride, dtype, M, K, w, ldb, sb, sums, bias, out, ldc, N, q, sa, zp, ws, ws_bytes, stream
+    good = [64, 256, 2, 4, 256, 64, 256, 64, 64, None, 64, 64, 64, 64, 64, 64, None, 0, None]
+    for at, value, code in ((0, None, -1), (5, None, -1), (7, None, -1), (10, None, -1), (13, None, -1), (14, None, -1), (15, None, -1), (2, 0, -1),
+                            (1, 128, -1), (6, 128, -1), (11, 32, -1), (3, -1, -1), (12, 0, -1)):
+        args = list(good)
+        args[at] = value
+        assert f(*args) == code, (at, value, _lib().sglamd_last_error())
+    long = list(good)
+    long[1] = long[4] = long[6] = 65552
+    assert f(*long) == -2
+    assert f(*[0 if i == 3 else v for i, v in enumerate(good)]) == 0
+
+
 def test_few_tokens_refuses():
     f, w = _lib().sglamd_fused_experts_few_tokens, _lib().sglamd_fused_experts_few_tokens_workspace
     assert w(4, 256, 8) == 4 * 8 * 256 * 4 and w(0, 256, 8) == 0 and w(1 << 40, 1 << 40, 8) == 0
