@@ -175,6 +175,43 @@ def test_a_block_of_them(dev):
     assert all(torch.equal(a, b) for a, b in zip((out, y, res2, moe), _run_block(p, x, res)))
 
 
+@pytest.mark.parametrize("static", [False, True])
+def test_an_fp8_block_of_them(dev, static):
+    """Norm -> fp8_scaled_mm -> SiLU -> fp8_scaled_mm -> norm -> e4m3 experts, per token and with given scales."""
+    from sglang_amd import fp8_scaled_mm
+    from sglang_amd.moe_runner.few_tokens import fused_experts_few_tokens
+    from sglang_amd.quantization.fused_row_quant import fused_rms_row_quant, silu_and_mul_row_quant
+
+    g = torch.Generator().manual_seed(3)
+    x, res = (torch.randn(6, 512, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+    gamma = (torch.rand(512, generator=g) + 0.5).to(dev)
+    w_up, w_down = ((torch.randn(*s, generator=g) * 100).clamp(-448, 448).to(F8).to(dev) for s in ((1280, 512), (512, 640)))
+    s_up, s_down = torch.full((1280, 1), 2e-4, device=dev), torch.full((512, 1), 2e-4, device=dev)
+    given = [torch.full((1,), v, device=dev) if static else None for v in (0.01, 0.004, 0.01)]
+
+    def fixed(scale):
+        return None if scale is None else float(scale)
+
+    def product(q, s, w, ws):
+        out = fp8_scaled_mm(q, w.t(), s, ws, torch.bfloat16)
+        a, b = q.cpu().float().double(), w.cpu().float().double()
+        scale = s.cpu().double() * ws.cpu().double().view(1, -1)
+        # 512 to 640 products, summed in 32 bits, times two scales
+        rl.check_rounded(out, (a @ b.t()) * scale, 3 * rl.U, (a.abs() @ b.abs().t()) * scale * 640 * rl.U)
+        return out
+
+    (q, s), _, r1 = fused_rms_row_quant(x, gamma, 1e-6, res=res, dtype_quant=F8, scale=given[0])
+    rl.check_codes(rl.rms(x.cpu(), gamma.cpu(), 1e-6, res.cpu())[1], rl.rms_error(512), q, s, None, fixed(given[0]))
+    mid = product(q, s, w_up, s_up)
+    q, s = silu_and_mul_row_quant(mid, dtype_quant=F8, scale=given[1])
+    rl.check_codes(rl.silu_mul(mid.cpu()), rl.silu_error(mid.cpu()), q, s, None, fixed(given[1]))
+    out = product(q, s, w_down, s_down)
+    (q, s), y, _ = fused_rms_row_quant(out, gamma, 1e-6, res=r1, dtype_quant=F8, scale=given[2], output_unquantized=True)
+    rl.check_rounded(y, rl.rms(out.cpu(), gamma.cpu(), 1e-6, r1.cpu())[1], rl.rms_error(512))
+    t = dict({k: v for k, v in _layer(dev, 6, 16, 2, 512, 256, False, 8).items() if not k.startswith("hidden")}, hidden_q=q, hidden_scale=s)
+    _check(fused_experts_few_tokens(**t), t)
+
+
 def test_captured_and_replayed(dev):
     """The run captured into two graphs that share a pool, replayed in turn on changing inputs with eager work between."""
     p = _with_sums(_block(dev))

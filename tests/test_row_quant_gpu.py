@@ -24,7 +24,7 @@ def _rows(g, *shape, dtype=torch.bfloat16, shift=0.0):
 
 
 # (teams of a wave, one workgroup form after the other, the value-by-value form: odd lengths and rows beyond 32768)
-ROW_SIZES = [(1, 1), (3, 7), (2, 8), (5, 24), (1, 128), (700, 512), (600, 1000), (37, 1536), (1, 7168), (530, 4096), (515, 8192),
+ROW_SIZES = [(1, 1), (3, 7), (2, 8), (5, 24), (1, 128), (700, 512), (600, 1000), (40, 1000), (600, 2000), (37, 1536), (1, 7168), (530, 4096), (515, 8192),
              (7, 8184), (9, 16384), (3, 28672), (2, 32776), (4, 4099)]
 
 
