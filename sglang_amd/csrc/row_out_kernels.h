@@ -164,19 +164,20 @@ __global__ __launch_bounds__(256) void row_out_any_kernel(RowOutArgs a) {
   }
 }
 
-constexpr int64_t ROW_OUT_MAX_HIDDEN = 512 * 8 * 8;  // the longest row that 512 lanes keep in registers
+constexpr int64_t ROW_OUT_MAX_HIDDEN = 512 * 8 * 8;  // the longest row that 512 or 1024 lanes keep in registers
 
 // Bound by memory with many rows (a copy's rate from some thousand rows of 4096 values: 4096 x 8192 with a residual 45 us, 5.2 TB/s;
-// SiLU of 4096 x [7168 | 7168] 29.5, 5.0), by one row's latency with few (one row of 7168 3.0 us, 2 of them a launch; SiLU
-// of 28672 values 5.9, the exponentials and reciprocals of a row on one CU).  Lanes x pieces per row: enough lanes that a row is short, few enough registers that a
-// CU holds several rows.  Best | next best, us, asymmetric codes (norm: e4m3), data from HBM:
+// SiLU of 4096 x [7168 | 7168] 29.5, 5.0), by one row's latency with few (one row of 7168 3.0 us, 2 of them a launch; SiLU of 28672
+// values 5.9, the exponentials and reciprocals of a row on one CU).  Lanes x pieces per row: enough lanes that a row is short, few
+// enough registers that a CU holds several rows.  Best | next best, us, asymmetric codes (norm: e4m3), data from HBM:
 //   a wave of 1 or 2 pieces  norm 16384 x 512 14.6 | 21.2 (256 x 1), SiLU 10.9 | 24.0; SiLU 16384 x 1024 17.6 | 28.7; norm 300 x 1024 3.5 against 3.1
 //   a wave of 4, plain rows  16384 x 2048 20.9 | 24.6 (256 x 1)
 //   256 x 1                  norm 16384 x 2048 43.9 | 48.4 (512 x 1), SiLU 32.7 | 34.6 (a wave of 4)
 //   512 x 1 (norm), 256 x 2  norm 1000 x 4096 8.7 | 9.3, SiLU 4096 x 4096 18.0 | 19.3, plain 16384 x 4096 38.4 | 48.1
 //   512 x 2, 256 x 4 (plain) norm 1000 x 8192 14.2 | 15.3 (256 x 4), SiLU 4096 x 7168 29.5 | 30.8 (256 x 4), plain 19.0 | 20.6 (512 x 2)
 //   1024 x 2                 norm 4096 x 14336 77 | 78 (512 x 4), SiLU 54.6 | 56.7, plain 33.9 | 34.1
-//   512 x 8                  SiLU 4096 x 18432 72 | 86 (1024 x 4: its registers leave a CU one row), 1000 x 28672 30.2 | 30.6
+//   512 x 8                  SiLU 3001 x 18432 53.8 | 55.0 (1024 x 4), 2000 x 28672 54.4 | 56.6
+//   1024 x 4                 norm 4096 x 18432 114.9 | 118.5 (512 x 8), SiLU to symmetric codes, which keep fewer registers, 72.8 | 76.0
 template <typename T, typename WT, int SRC, int QK>
 static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
   const dim3 grid((unsigned)a.rows);
@@ -197,7 +198,7 @@ static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
     else if (nvec <= 512) SGLAMD_ROW_OUT((RMS ? 512 : 256), (RMS ? 1 : 2));
     else if (nvec <= 1024) SGLAMD_ROW_OUT((PLAIN ? 256 : 512), (PLAIN ? 4 : 2));
     else if (nvec <= 2048) SGLAMD_ROW_OUT(1024, 2);
-    else SGLAMD_ROW_OUT(512, 8);
+    else SGLAMD_ROW_OUT((!RMS && QK == ROW_TO_ASYM ? 512 : 1024), (!RMS && QK == ROW_TO_ASYM ? 8 : 4));
 #undef SGLAMD_ROW_OUT
 #undef SGLAMD_ROW_TEAM
   }
