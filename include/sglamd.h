@@ -242,7 +242,7 @@ int sglamd_int8_row_linear(const void* x, int64_t x_row_stride, int dtype, int64
                            int64_t ldc, int64_t N, void* q, float* sa, int32_t* zp, void* workspace,
                            int64_t workspace_bytes, void* stream);
 
-/* sums[n] = sum over k of b[n, k], b int8 [N, K] with rows of ldb bytes, any K below 2^24 and any alignment. */
+/* sums[n] = sum over k of b[n, k], b int8 [N, K] with rows of ldb bytes, any N below 2^26, K below 2^24 and alignment. */
 int sglamd_int8_weight_sums(const void* b, int64_t ldb, int64_t N, int64_t K, int32_t* sums, void* stream);
 
 /* Optional scratch for the three GEMM entry points above.  For shapes whose tile grid alone cannot fill the
@@ -461,15 +461,16 @@ int sglamd_fused_rms_fp8_group_quant(const void* x1, int64_t x1_row_stride, cons
  *              zp = rint(-128 - lo / scale);  code = clamp(rint(y * (1 / scale)) + zp, -128, 127);  y is scale * (code - zp)
  * output_q [rows, hidden], output_s fp32 [rows] (a fixed scale is repeated), output_zp int32 [rows] or NULL.  Rows may have
  * any length, stride (in elements, 0 included) and alignment; lengths that are multiples of 8, at most 32768, in 16-byte
- * aligned rows are read once in 16-byte pieces, all others value by value, twice.  Outputs overlap no input.  A row that
- * holds a NaN or an infinity gets a scale that is NaN or infinite (a fixed scale: NaN codes), so that it stays visible
- * behind the product.
+ * aligned rows are read once in 16-byte pieces, all others value by value, twice.  Outputs overlap no input.  A row of y that
+ * holds a NaN or an infinity gets a scale that is NaN or infinite, so that it stays visible behind the product.  With a fixed
+ * scale a NaN is e4m3's NaN and an infinity saturates; a row whose sum of squares is not finite is all NaN.  e4m3 rows whose
+ * largest value is below 1e-36 keep fewer bits than others, and zeros.
  *
  * sglamd_fused_rms_row_quant: v = f32(x) + f32(res), res_out = cast(v), y = v * weight * (1 / sqrt(mean(v^2) + eps)), the
  *   optional output y = cast(y).  x, res, y, res_out in dtype (F16/BF16), y and res_out [rows, hidden] contiguous; weight
  *   [hidden] of F32 or dtype; res and res_out go together (NULL: none).  A sum of squares beyond fp32 counts as infinite.
  *   Stands beside sglamd_fused_rms_fp8_group_quant for the row-scaled products (sglamd_fp8_scaled_mm, sglamd_int8_scaled_mm).
- * sglamd_silu_mul_row_quant: y = gate / (1 + exp(-gate)) * up, x rows of [gate | up], 2 * hidden values, F16/BF16.
+ * sglamd_silu_mul_row_quant: y = gate / (1 + exp(-gate)) * up, x rows of [gate | up], 2 * hidden values, F16/BF16.  Gates below -87 give 0.
  * sglamd_per_token_quant_int8_asym: y = x, with zero points; F32/F16/BF16. */
 int sglamd_fused_rms_row_quant(const void* x, int64_t x_row_stride, const void* res, int64_t res_row_stride,
                                const void* weight, float eps, const float* fixed_scale, int64_t rows, int64_t hidden,
@@ -486,8 +487,8 @@ int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_stride, int dt
  *   h = x_scale[t] * w13_scale[e] * (x[t] . w13[e]) (+ b13[e]);  a = silu(gate) * up in fp32, in 8 bits per (token, expert)
  *   pair by the symmetric formulas above;  out[t] = cast( routed_scaling_factor * sum over the token's pairs, in their order, of
  *   topk_weights * (a_scale * w2_scale[e] * (a . w2[e]) (+ b2[e])) ).
- * Against sglamd_fused_moe_layer it takes quantised rows and rounds nothing to 16 bits on the way.  Bits depend on neither
- * the order of arrivals nor the launch.
+ * Against sglamd_fused_moe_layer it takes quantised rows and rounds nothing to 16 bits on the way.  The same call gives
+ * the same bits.
  * x [M, H] e4m3fn or int8 (q_dtype), contiguous; w13 [E, 2 * I, H] (gate rows, then up rows), w2 [E, H, I] of that type;
  * w13_scale fp32 [E, 2 * I], w2_scale [E, H]; b13, b2 optional, shaped like the scales, in out_dtype (F16/BF16);
  * topk_weights fp32 [M, topk], topk_ids [M, topk] int32 or int64: pairs whose id is outside [0, E) contribute nothing, an

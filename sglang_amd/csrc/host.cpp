@@ -716,8 +716,9 @@ Tensor int8_linear(const Tensor& x, const Tensor& weight, const Tensor& ws, cons
   const int64_t q = sc.take(m * k), sa = sc.take(4 * m), zp = sums ? sc.take(4 * m) : 0;
   const int64_t wb = sglamd_gemm_workspace_bytes(m, n, k), wp = sc.take(wb > 0 ? wb : 0);
   sc.allocate(x);
-  // (rows without zero points are quantised from contiguous, 16-byte aligned ones)
-  const Tensor rows = sums || (x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0) ? x : x.clone(at::MemoryFormat::Contiguous);
+  // (rows without zero points are quantised from contiguous, 16-byte aligned ones; no row shares values with another)
+  const bool as_they_lie = sums ? m == 1 || x.stride(0) >= k : x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0;
+  const Tensor rows = as_they_lie ? x : x.clone(at::MemoryFormat::Contiguous);
   check(sglamd_int8_row_linear(rows.data_ptr(), ld(rows, 0), tag(t), m, k, weight.data_ptr(), ld(weight, 1), ws.data_ptr<float>(),
                                sums ? sums->data_ptr<int32_t>() : nullptr, bias ? bias->data_ptr() : nullptr, out.data_ptr(), n, n, sc.at(q),
                                (float*)sc.at(sa), sums ? (int32_t*)sc.at(zp) : nullptr, wb > 0 ? sc.at(wp) : nullptr, wb, stream_of(x)));

@@ -296,7 +296,7 @@ __device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_
     mul = 127.0f / amax;
   } else {
     scale = amax0 / 448.0f;
-    mul = scale == 0.f ? 0.f : 1.0f / scale;
+    mul = fp8_row_multiplier(1.0f, scale);
   }
   const RowScale o = {scale, mul, 0.f, 1.f};
   auto put = [&](int c, const v4f& q) {

@@ -68,8 +68,8 @@ extern "C" int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_str
 extern "C" int sglamd_int8_weight_sums(const void* b, int64_t ldb, int64_t N, int64_t K, int32_t* sums, void* stream) {
   const char* op = "int8_weight_sums";
   SGLAMD_REQUIRE(b && sums, SGLAMD_EINVAL, "%s: null pointer", op);
-  SGLAMD_REQUIRE(N >= 0 && N < (1ll << 31) && K > 0 && K < (1ll << 24), SGLAMD_EINVAL, "%s: bad sizes N=%lld K=%lld", op, (long long)N,
-                 (long long)K);  // (sums of fewer than 2^24 codes stay inside 32 bits)
+  SGLAMD_REQUIRE(N >= 0 && N < (1ll << 26) && K > 0 && K < (1ll << 24), SGLAMD_EINVAL, "%s: bad sizes N=%lld K=%lld", op, (long long)N,
+                 (long long)K);  // (a launch holds fewer than 2^32 lanes; sums of fewer than 2^24 codes stay inside 32 bits)
   SGLAMD_REQUIRE(ldb >= K, SGLAMD_EINVAL, "%s: leading dimension smaller than the row", op);
   if (N == 0) return SGLAMD_OK;
   const bool pieces = K % 16 == 0 && ldb % 16 == 0 && aligned_to(b, 16);

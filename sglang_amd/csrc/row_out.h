@@ -114,7 +114,7 @@ __device__ __forceinline__ RowStats row_stats_block(RowStats t, uint32_t* red) {
 template <int SRC, int QK>
 __device__ __forceinline__ void row_stats_add(RowStats& t, float y) {
   if (QK == ROW_TO_ASYM) {
-    // (a NaN compares as neither, and is caught by the sum of squares, or by row_stats_poison)
+    // (a NaN compares as neither, and is caught by row_stats_poison)
     t.hi = __float_as_uint(fmaxf(__uint_as_float(t.hi), y));
     t.lo = __float_as_uint(fmaxf(__uint_as_float(t.lo), -y));
   } else {
@@ -124,6 +124,13 @@ __device__ __forceinline__ void row_stats_add(RowStats& t, float y) {
 // Asymmetric codes: `poison` is a sum of 0 * y, NaN exactly where a value is not finite.
 __device__ __forceinline__ void row_stats_poison(RowStats& t, float poison) {
   if (poison != 0.f) t.hi = 0x7fc00000u;
+}
+
+// What turns a value into an e4m3 code's: finite, so that a zero in a row whose scale has no reciprocal in 32 bits (values below
+// 1e-36) stays a zero.
+__device__ __forceinline__ float fp8_row_multiplier(float r, float scale) {
+  const float mul = scale == 0.f ? 0.f : r / scale;
+  return mul > 3.4028234664e38f ? 3.4028234664e38f : mul;  // (a NaN stays one)
 }
 
 // How the values of a row become codes: code = convert(value * mul) (asymmetric: + zp).
@@ -143,7 +150,7 @@ __device__ __forceinline__ RowScale row_scale(const RowOutArgs& a, const RowStat
   const float hi = __uint_as_float(t.hi) * o.r;
   if constexpr (QK == ROW_TO_FP8) {
     o.scale = a.fixed ? *a.fixed : hi / 448.0f;
-    o.mul = o.scale == 0.f ? 0.f : o.r / o.scale;
+    o.mul = fp8_row_multiplier(o.r, o.scale);
   } else if constexpr (QK == ROW_TO_INT8) {
     const float amax = hi > 1e-10f || hi != hi ? hi : 1e-10f;
     o.scale = amax / 127.0f;

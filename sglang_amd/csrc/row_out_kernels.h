@@ -86,10 +86,10 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       row_stats_add<SRC, QK>(t, u[k][j]);
-      if (QK == ROW_TO_ASYM && SRC != ROW_RMS) poison = fmaf(u[k][j], 0.f, poison);
+      if (QK == ROW_TO_ASYM) poison = fmaf(u[k][j], 0.f, poison);
     }
   }
-  if (QK == ROW_TO_ASYM && SRC != ROW_RMS) row_stats_poison(t, poison);
+  if (QK == ROW_TO_ASYM) row_stats_poison(t, poison);
   t = TEAM ? row_stats_wave<SRC, QK>(t) : row_stats_block<SRC, QK>(t, red);
   const RowScale o = row_scale<SRC, QK>(a, t);
   if (row >= a.rows) return;
@@ -112,15 +112,23 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
   }
 }
 
+// A launch holds fewer than 2^32 lanes in each dimension: workgroups beyond 2^20 go into the second one.
+constexpr int ROW_OUT_GRID_BITS = 20;
+__device__ __forceinline__ int64_t row_out_block() { return ((int64_t)blockIdx.y << ROW_OUT_GRID_BITS) + blockIdx.x; }
+static inline dim3 row_out_grid(int64_t blocks) {
+  const int64_t most = 1ll << ROW_OUT_GRID_BITS;
+  return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)ceil_div(blocks, most));
+}
+
 template <typename T, typename WT, int SRC, int QK, int NT, int NV>
 __global__ __launch_bounds__(NT) void row_out_kernel(RowOutArgs a) {
   __shared__ uint32_t red[48];
-  row_out_body<T, WT, SRC, QK, NV, 0>(a, blockIdx.x, red);
+  row_out_body<T, WT, SRC, QK, NV, 0>(a, row_out_block(), red);
 }
 // Short rows, a wave each.
 template <typename T, typename WT, int SRC, int QK, int NV>
 __global__ __launch_bounds__(256) void row_out_team_kernel(RowOutArgs a) {
-  row_out_body<T, WT, SRC, QK, NV, 64>(a, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), nullptr);
+  row_out_body<T, WT, SRC, QK, NV, 64>(a, row_out_block() * 4 + (threadIdx.x >> 6), nullptr);
 }
 
 // Any row length and alignment, 32-bit rows: a workgroup per row, values one by one, the row read twice (the second time
@@ -129,7 +137,8 @@ template <typename T, typename WT, int SRC, int QK>
 __global__ __launch_bounds__(256) void row_out_any_kernel(RowOutArgs a) {
   typedef typename T::storage S;
   __shared__ uint32_t red[48];
-  const int64_t row = blockIdx.x;
+  const int64_t row = row_out_block();
+  if (row >= a.rows) return;
   const S* x = (const S*)a.x + row * a.x_stride;
   const S* res = a.res ? (const S*)a.res + row * a.res_stride : nullptr;
   auto sum_at = [&](int64_t i) -> float { return T::to_f32(x[i]) + (res ? T::to_f32(res[i]) : 0.f); };
@@ -148,9 +157,9 @@ __global__ __launch_bounds__(256) void row_out_any_kernel(RowOutArgs a) {
     }
     const float u = value_at(i);
     row_stats_add<SRC, QK>(t, u);
-    if (QK == ROW_TO_ASYM && SRC != ROW_RMS) poison = fmaf(u, 0.f, poison);
+    if (QK == ROW_TO_ASYM) poison = fmaf(u, 0.f, poison);
   }
-  if (QK == ROW_TO_ASYM && SRC != ROW_RMS) row_stats_poison(t, poison);
+  if (QK == ROW_TO_ASYM) row_stats_poison(t, poison);
   t = row_stats_block<SRC, QK>(t, red);
   const RowScale o = row_scale<SRC, QK>(a, t);
   if (threadIdx.x == 0) {
@@ -180,7 +189,7 @@ constexpr int64_t ROW_OUT_MAX_HIDDEN = 512 * 8 * 8;  // the longest row that 512
 //   1024 x 4                 norm 4096 x 18432 114.9 | 118.5 (512 x 8), SiLU to symmetric codes, which keep fewer registers, 72.8 | 76.0
 template <typename T, typename WT, int SRC, int QK>
 static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
-  const dim3 grid((unsigned)a.rows);
+  const dim3 grid = row_out_grid(a.rows);
   if (!pieces) {
     hipLaunchKernelGGL((row_out_any_kernel<T, WT, SRC, QK>), grid, dim3(256), 0, st, a);
     return;
@@ -189,7 +198,7 @@ static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
     const int64_t nvec = a.hidden >> 3;
     const bool many = a.rows >= 2 * (int64_t)device_cus();
     constexpr bool RMS = SRC == ROW_RMS, PLAIN = SRC == ROW_PLAIN;
-#define SGLAMD_ROW_TEAM(NV) hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, NV>), dim3((unsigned)ceil_div(a.rows, 4)), dim3(256), 0, st, a)
+#define SGLAMD_ROW_TEAM(NV) hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, NV>), row_out_grid(ceil_div(a.rows, 4)), dim3(256), 0, st, a)
 #define SGLAMD_ROW_OUT(NT, NV) hipLaunchKernelGGL((row_out_kernel<T, WT, SRC, QK, NT, NV>), grid, dim3(NT), 0, st, a)
     if (nvec <= 64) SGLAMD_ROW_TEAM(1);
     else if (nvec <= 128 && (many || !RMS)) SGLAMD_ROW_TEAM(2);

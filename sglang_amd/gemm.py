@@ -15,7 +15,7 @@ def int8_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias=None):
 
 
 def int8_scaled_mm_azp(mat_a, mat_b, scales_a, scales_b, out_dtype, azp, weight_sums, bias=None):
-    """int8_scaled_mm of rows with a zero point each: (mat_a - azp) x mat_b.  azp int32, one per row of A; weight_sums int32,
+    """int8_scaled_mm of rows with a zero point each: (mat_a - azp) x mat_b.  azp int32, one per row of A, in [-128, 127]; weight_sums int32,
     the sums of mat_b over K (quantization.int8_utils.int8_weight_sums).  K <= 65536."""
     return ops._C.int8_scaled_mm_azp(mat_a, mat_b, scales_a, scales_b, out_dtype, azp, weight_sums, bias)
 

@@ -11,8 +11,8 @@ With y the row before its codes, all in float32 and not rounded on the way:
                        zp = round(-128 - lo / scale);  code = clamp(round(y / scale) + zp, -128, 127)
 
 The codes are (q, scale) or (q, scale, zp): q like the row, scale float32 [M, 1], zp int32 [M, 1]; y is about
-scale * (q - zp).  A row that holds a NaN or an infinity gets a scale that is NaN or infinite (a given scale: NaN codes).
-Rows may have any length and stride; multiples of 8 in 16-byte aligned rows are the fast ones.  There is no gradient."""
+scale * (q - zp).  A row of y that holds a NaN or an infinity gets a scale that is NaN or infinite; with a given scale a NaN stays
+a NaN code and an infinity saturates (behind the norm the whole row is NaN).  Rows may have any length and stride; multiples of 8 in 16-byte aligned rows are the fast ones.  There is no gradient."""
 from typing import Optional, Tuple
 
 import torch

@@ -50,6 +50,18 @@ def test_layer(dev, int8, m, e, topk, h, i):
     assert torch.equal(out, fused_experts_few_tokens(**t))
 
 
+def test_intermediate_rows_whose_scale_has_no_reciprocal(dev):
+    """Values of some 1e-38 and zeros between the products: 256 terms of at most 448 * 1e-36, and nothing that is not finite."""
+    from sglang_amd.moe_runner.few_tokens import fused_experts_few_tokens
+
+    t = _layer(dev, 2, 4, 2, 512, 256, False, 3)
+    t["w1"].view(torch.int8)[:, 256 + 5] = 0
+    t["w1_scale"][:, 256:] = 1e-40
+    t["w2_scale"][:] = 1.0
+    out = fused_experts_few_tokens(**t).cpu()
+    assert torch.isfinite(out).all() and (out.abs() <= 2 * 256 * 448 * 1e-36).all()
+
+
 @pytest.mark.parametrize("int8", [True, False])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_biases_factor_and_types(dev, int8, dtype):

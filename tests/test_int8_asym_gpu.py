@@ -183,6 +183,10 @@ def test_linear_of_views_one_scale_and_no_rows(dev):
     for view in (wide[:, 8:1032], wide[:, 1:1025], wide[::2, :1024]):
         for asym in (None, sums):
             assert torch.equal(apply_int8_linear(view, w.t(), sb, asym), apply_int8_linear(view.contiguous(), w.t(), sb, asym))
+    line = wide.view(-1)
+    for view in (wide[:1, :1024].expand(5, 1024), line.as_strided((4, 1024), (8, 1)), line.as_strided((1, 1024), (1, 1)), wide[:1, :1024].expand(40, 1024)):
+        for asym in (None, sums):
+            assert torch.equal(apply_int8_linear(view, w.t(), sb, asym), apply_int8_linear(view.contiguous(), w.t(), sb, asym))
     one = torch.full((1,), 0.01, device=dev)
     x = wide[:, :1024].contiguous()
     assert torch.equal(apply_int8_linear(x, w.t(), one, sums), apply_int8_linear(x, w.t(), one.expand(64).contiguous(), sums))

@@ -115,6 +115,48 @@ def test_rows_with_a_nan_or_an_infinity_stay_visible(dev, hidden, bad):
                 assert finite.tolist() == [True, True, False, True], kind
 
 
+@pytest.mark.parametrize("hidden", [64, 1024, 8192, 333])
+@pytest.mark.parametrize("weight,value", [(float("nan"), 1.0), (float("inf"), 1.0), (float("inf"), 0.0)])
+def test_a_norm_with_a_bad_weight_stays_visible(dev, hidden, weight, value):
+    from sglang_amd.quantization.fused_row_quant import fused_rms_row_quant
+
+    x = _rows(torch.Generator().manual_seed(hidden), 3, hidden)
+    w = torch.ones(hidden)
+    w[hidden // 2 + 1], x[:, hidden // 2 + 1] = weight, value
+    for kind in ("fp8", "int8", "asym"):
+        assert not torch.isfinite(fused_rms_row_quant(x.to(dev), w.to(dev), 1e-6, **_options(kind, dev))[0][1]).any(), kind
+
+
+@pytest.mark.parametrize("hidden", [64, 1024, 8192, 333])
+def test_values_whose_scale_has_no_reciprocal(dev, hidden):
+    """Zeros stay zeros, and what is lost is below 1e-36 times what the norm multiplies by (1 / sqrt(eps))."""
+    from sglang_amd.quantization.fused_row_quant import fused_rms_row_quant, silu_and_mul_row_quant
+
+    x = torch.zeros(2, hidden, dtype=torch.bfloat16)
+    x[0, ::3], x[1, 5], x[1, 7] = 1e-38, -3e-38, 1e-36
+    up = torch.cat([torch.full_like(x, 4.0), x], dim=1)
+    (q, s), _, _ = fused_rms_row_quant(x.to(dev), torch.ones(hidden, device=dev), 1e-6, dtype_quant=F8)
+    qs, ss = silu_and_mul_row_quant(up.to(dev), dtype_quant=F8)
+    for codes, scale, y, lost in ((q, s, rl.rms(x, torch.ones(hidden), 1e-6)[1], 2e-33), (qs, ss, rl.silu_mul(up), 1e-35)):
+        c = codes.cpu().float()
+        assert (c[x == 0] == 0).all()
+        assert ((c.double() * scale.cpu().double() - y).abs() <= lost).all()
+
+
+@pytest.mark.parametrize("rows,hidden", [((1 << 22) + 3, 8), ((1 << 20) + 1, 1032), ((1 << 24) + 5, 3)])
+def test_more_rows_than_one_grid_dimension_holds(dev, rows, hidden):
+    from sglang_amd.quantization.int8_kernel import per_token_quant_int8_asym
+
+    g = torch.Generator().manual_seed(hidden)
+    some = _rows(g, 1009, hidden, dtype=torch.float16, shift=0.5).to(dev)
+    x = some.repeat(rows // 1009 + 1, 1)[:rows]
+    want = per_token_quant_int8_asym(some)
+    for got, part in zip(per_token_quant_int8_asym(x), want):
+        assert got.shape[0] == rows
+        whole = rows // 1009 * 1009
+        assert (got[:whole].view(-1, 1009, got.shape[1]) == part).all() and torch.equal(got[whole:], part[:rows - whole])
+
+
 def test_the_other_rows_do_not_see_a_bad_one(dev):
     from sglang_amd.quantization.fused_row_quant import silu_and_mul_row_quant
 
