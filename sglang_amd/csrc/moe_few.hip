@@ -17,13 +17,14 @@
 //     are summed in the pairs' order, so the sum over a token's experts needs neither atomics nor a launch.
 //
 // Measured (kernels, us; in brackets a bare read of the weights' bytes): 6 of 64 int8 experts of 4096 x 1536, one token, 15.2 + 10.6
-// (16.4); 8 of 128 e4m3 experts of 2048 x 768, three tokens, 15.1 + 14.7 (15.5); 8 of 256 of 7168 x 2048, one token 38.7 + 23.2 (51),
+// (16.4); 8 of 128 e4m3 experts of 2048 x 768, three tokens, 15.1 + 11.0 (15.5); 8 of 256 of 7168 x 2048, one token 38.7 + 23.2 (51),
 // four 133 + 80 (195).  Large layers run at the rate of a read; small ones wait for two launches, and in each for a chain of ids, rows
 // and first weights, some 4 us a launch.
 // Tried: the second launch's rows quantised by the workgroup together, behind a barrier (four tokens of the large layer 80 -> 89: all
-// waves quantise at once and all stream at once); sixteen waves to its workgroups (registers spill, 14 -> 22); a wave's next group
-// requested under the results of the one before (80 -> 97 where it spills, 78 -> 80 elsewhere); the first launch's rows from L1 instead of LDS
-// (their loads return behind the weights that were requested before them: 4096 x 1408, four tokens, 20.6 against 13.3).
+// waves quantise at once and all stream at once); sixteen waves to all its workgroups (registers spill, or fewer are left for the loads:
+// four tokens of the large layer 205 -> 214, both launches); a wave's next group requested under the results of the one before
+// (80 -> 97 where it spills, 78 -> 80 elsewhere); the first launch's rows from L1 instead of LDS (their loads return behind the weights
+// that were requested before them: 4096 x 1408, four tokens, 20.6 against 13.3).
 #include <algorithm>
 
 #include "row_out.h"
@@ -47,7 +48,8 @@ struct FewArgs {
 
 constexpr int FEW_MAX_PAIRS = 64;  // one lane each
 constexpr int FEW_MAX_HIDDEN = 32768, FEW_MAX_INTER = 16384;  // a row in LDS, eight of them
-constexpr int FEW_DOWN_WAVES = 8;
+constexpr int FEW_DOWN_WAVES = 8;      // of the second launch, twice as many on up to FEW_SHORT_INTER values
+constexpr int FEW_SHORT_INTER = 1024;
 constexpr int FEW_LDS = 64 * 1024;  // what several rows for a pass may take, two workgroups to a CU
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -268,16 +270,16 @@ __global__ __launch_bounds__(256) void few_up_kernel(FewArgs a) {
   }
 }
 
-// Row `pair` of a, quantised into LDS; returns its scale.  Up to 2048 values stay in registers between the maximum and the
+// Row `pair` of a, quantised into LDS; returns its scale.  Up to KEEP * 256 values stay in registers between the maximum and the
 // codes, longer rows are read again.
-constexpr int FEW_KEEP = 8;
-__device__ __forceinline__ void few_act_load(const FewArgs& a, int pair, int lane, v4f (&v)[FEW_KEEP]) {
+template <int KEEP>
+__device__ __forceinline__ void few_act_load(const FewArgs& a, int pair, int lane, v4f (&v)[KEEP]) {
   const v4f* src = (const v4f*)(a.act + (int64_t)pair * a.I);
 #pragma unroll
-  for (int k = 0; k < FEW_KEEP; k++) v[k] = src[min(lane + k * 64, (a.I >> 2) - 1)];  // (repeats change no maximum)
+  for (int k = 0; k < KEEP; k++) v[k] = src[min(lane + k * 64, (a.I >> 2) - 1)];  // (repeats change no maximum)
 }
-template <bool INT8>
-__device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_t* dst, int lane, const v4f (&v)[FEW_KEEP]) {
+template <bool INT8, int KEEP>
+__device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_t* dst, int lane, const v4f (&v)[KEEP]) {
   const v4f* src = (const v4f*)(a.act + (int64_t)pair * a.I);
   const int chunks = a.I >> 2;
   uint32_t top = 0;
@@ -286,8 +288,8 @@ __device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_
     for (int j = 0; j < 4; j++) top = umax(top, __float_as_uint(c[j]) & 0x7fffffffu);
   };
 #pragma unroll
-  for (int k = 0; k < FEW_KEEP; k++) take(v[k]);
-  for (int c = lane + FEW_KEEP * 64; c < chunks; c += 64) take(src[c]);
+  for (int k = 0; k < KEEP; k++) take(v[k]);
+  for (int c = lane + KEEP * 64; c < chunks; c += 64) take(src[c]);
   const float amax0 = __uint_as_float(wave_umax(top));
   float scale, mul;
   if constexpr (INT8) {
@@ -304,15 +306,15 @@ __device__ __forceinline__ float few_quantise(const FewArgs& a, int pair, uint8_
     *(uint32_t*)(dst + 4 * c) = row_codes4<INT8 ? ROW_TO_INT8 : ROW_TO_FP8>(f, o);
   };
 #pragma unroll
-  for (int k = 0; k < FEW_KEEP; k++)
+  for (int k = 0; k < KEEP; k++)
     if (lane + k * 64 < chunks) put(lane + k * 64, v[k]);
-  for (int c = lane + FEW_KEEP * 64; c < chunks; c += 64) put(c, src[c]);
+  for (int c = lane + KEEP * 64; c < chunks; c += 64) put(c, src[c]);
   return scale;
 }
 
 // grid: tiles of 2 * 64 / LPR output columns, a group to a wave in turn.  LDS: RMAX rows of I codes for each wave.
-template <bool INT8, typename OT, int RMAX, int LPR>
-__global__ __launch_bounds__(512) void few_down_kernel(FewArgs a) {
+template <bool INT8, typename OT, int RMAX, int LPR, int KEEP, int NT>
+__global__ __launch_bounds__(NT) void few_down_kernel(FewArgs a) {
   typedef typename OT::storage OS;
   typedef typename std::conditional<INT8, int, float>::type acc_t;
   constexpr int COLS = 64 / LPR, S = few_batch(RMAX, LPR);
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs a) {
     return {0, 0};
   };
   // A group's first row, then its first weights: loads return in the order of their requests.
-  v4f row[FEW_KEEP];
+  v4f row[KEEP];
   FewBatch<S> batch;
   const uint8_t *w0, *w1;
   auto request = [&](const FewGroup& g) {
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(512) void few_down_kernel(FewArgs a) {
       scale[r] = 0.f;
       if (r >= count) continue;
       if (r > 0) few_act_load(a, pairs[r], lane, row);
-      scale[r] = few_quantise<INT8>(a, pairs[r], codes + r * a.I, lane, row);
+      scale[r] = few_quantise<INT8, KEEP>(a, pairs[r], codes + r * a.I, lane, row);
     }
     // (the rows are this wave's own: its LDS instructions run in order)
     asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
@@ -419,10 +421,10 @@ static int few_start_up(const FewArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(kern, grid, dim3(256), smem, st, a);
   return check_launch("few_up");
 }
-template <bool INT8, typename OT, int RMAX, int LPR>
-static int few_start_down(const FewArgs& a, hipStream_t st) {
-  auto kern = few_down_kernel<INT8, OT, RMAX, LPR>;
-  const int waves = std::min(a.M * a.topk, FEW_DOWN_WAVES), smem = waves * RMAX * a.I;
+template <bool INT8, typename OT, int RMAX, int LPR, int WAVES>
+static int few_start_down_waves(const FewArgs& a, hipStream_t st) {
+  auto kern = few_down_kernel<INT8, OT, RMAX, LPR, WAVES == FEW_DOWN_WAVES ? 8 : FEW_SHORT_INTER / 256, 64 * WAVES>;
+  const int waves = std::min(a.M * a.topk, WAVES), smem = waves * RMAX * a.I;
   if (smem > 56 * 1024) {
     static SmemAttrOnce attr;
     const hipError_t e = raise_dynamic_smem(attr, (const void*)kern, smem);
@@ -430,6 +432,17 @@ static int few_start_down(const FewArgs& a, hipStream_t st) {
   }
   hipLaunchKernelGGL(kern, dim3((unsigned)ceil_div(a.H, 2 * (64 / LPR))), dim3(64 * waves), smem, st, a);
   return check_launch("few_down");
+}
+
+// Eight waves; sixteen of at most two rows a pass where the pairs take more than one turn on rows so short that the registers of
+// sixteen suffice, and the chain of a turn counts, not its bytes (8 | 16 waves, both launches: 8 of 128 experts of 2048 x 768, three tokens
+// 30.0 | 26.2 us, eight 63.6 | 53.9; 6 of 64 of 2048 x 1024, four 33.0 | 30.6; 8 of 64 of 1024 x 512, eight 32.9 | 27.6; where eight lanes
+// read a row they spill: 8 of 64 of 4096 x 1024, three 57.5 | 66.8, of one row a pass 58.8).
+template <bool INT8, typename OT, int RMAX, int LPR>
+static int few_start_down(const FewArgs& a, hipStream_t st) {
+  if constexpr (LPR > 8)
+    if (a.M * a.topk > FEW_DOWN_WAVES && a.I <= FEW_SHORT_INTER) return few_start_down_waves<INT8, OT, RMAX == 1 ? 1 : 2, LPR, 2 * FEW_DOWN_WAVES>(a, st);
+  return few_start_down_waves<INT8, OT, RMAX, LPR, FEW_DOWN_WAVES>(a, st);
 }
 
 template <bool INT8, typename OT>

@@ -265,3 +265,13 @@ def test_on_two_streams_at_once(dev):
                 got.append(_run_block(p, *i))
     torch.cuda.synchronize()
     assert all(torch.equal(u, v) for n, o in enumerate(got) for u, v in zip(o, want[n % 2]))
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("m,e,topk,h,i", [(3, 40, 8, 2048, 768), (1, 80, 64, 1024, 1024), (9, 6, 1, 528, 1024), (6, 3, 10, 80, 16), (5, 64, 2, 4064, 1008)])
+def test_more_pairs_than_eight_waves_take_at_once(dev, int8, m, e, topk, h, i):
+    from sglang_amd.moe_runner.few_tokens import fused_experts_few_tokens
+
+    t = _layer(dev, m, e, topk, h, i, int8, m * e + i, bias=torch.bfloat16)
+    print(f"few tokens {m} x {topk} of {e}, {h} x {i}, int8 {int8}", flush=True)
+    _check(fused_experts_few_tokens(**t), t)
