@@ -182,19 +182,21 @@ static inline int dense_plan(bool block, int64_t M, int64_t N, int64_t K, int32_
 }
 
 // The row modes' tile kernel also takes a K that is not a multiple of 128, from 512 up: 8192 x 4112 at 100 / 300 / 1000 rows
-// 43 / 45 / 60 -> 21 / 32 / 46 us (4096: 20 / 23 / 39), 28672 x 4112 at 2048 rows 407 -> 281.  Shorter sums are a launch of
-// 12 to 17 us either way and stay with the generic kernel.
+// 43 / 45 / 60 -> 21 / 32 / 46 us (4096: 20 / 23 / 39), 28672 x 4112 at 2048 rows 407 -> 281.  Shorter sums stay with the generic
+// kernel without zero points, whose last bits with a bias are its own; with them the tile kernel takes every K beyond 64 rows (300 x 4096
+// x 272 19.5 -> 9.2 us, 65 x 64 x 16 14.9 -> 7.6, 992 x 25920 x 64 77 -> 30, 4096 x 4096 x 496 52 -> 25).
 template <int MODE, typename OT>
 static int dispatch_dense(const GemmArgs& g, hipStream_t st, void* workspace, int64_t workspace_bytes,
                           bool may_split = true) {
   RAN(SGLAMD_KERNEL_STREAMING);
-  const bool big = gemm8_big_ok(g, !gemm_is_block(MODE) && g.K >= 512);
+  const bool any_k = g.K >= 512 || (out_zero_point<OT> && g.M > 64);
+  const bool big = gemm8_big_ok(g, !gemm_is_block(MODE) && any_k);
   const int wgs = gemm_is_block(MODE) ? persist_workgroups() : 0;
   const int nkb = g.K >> 7;
   const bool persistent = wgs > 0 && (wgs & 7) == 0 && !(nkb & 1) && nkb >= 4 && nkb <= GEMM8_PERSIST_USE_MAX_KB;
   const int tiles_256 = persistent ? (MODE == GEMM_BLOCK_FP8 && g.scales_pow2 ? 2 : 1) : 0;
   strip_last_shape = skinny_last_shape = 0;
-  if (big && may_split && g.M > 16) {
+  if (big && may_split && g.M > 16 && (g.K >= 512 || (g.K & 127) == 0)) {
     const DenseChoice choice = dense_choice(g.M, g.N, g.K);
     const StripPlan plan = strip_plan_for<OT>(choice.strip, g.M);
     if (choice.row_tile && gemm8_skinny_ok(g, g.M)) {

@@ -8,6 +8,7 @@ from .base import (  # noqa: F401
     TritonMoeQuantInfo,
     fused_experts_none_to_triton,
 )
+from .few_tokens import fused_experts_few_tokens, takes_few_tokens  # noqa: F401
 from .fused_moe import (  # noqa: F401
     fused_experts,
     fused_experts_impl,

@@ -6,6 +6,7 @@ from . import row_layers as rl
 
 pytestmark = pytest.mark.gpu
 STREAMING, TILE64, TILE128, TILE256, GENERIC, WIDE, TILE192, STRIP = 1, 2, 3, 4, 6, 8, 9, 10
+TILES = (TILE64, TILE128, TILE256, TILE192)
 
 
 def _operands(dev, m, n, k, seed, pitch=0):
@@ -25,7 +26,10 @@ SIZES = [
     (80, 28672, 4096, STRIP), (97, 28672, 4096, STRIP), (128, 28672, 4096, STRIP), (128, 57344, 2048, None), (120, 7168, 16384, None),
     (100, 20480, 8192, None), (64, 8192, 28672, None), (130, 4096, 4096, None), (200, 8192, 8192, None), (300, 2048, 2048, None),
     (300, 8192, 28672, None), (700, 8192, 1024, None), (512, 36864, 1024, None), (1100, 4096, 1536, None), (2048, 8192, 512, None),
-    (100, 8192, 4112, None), (65, 24, 48, GENERIC), (130, 200, 400, GENERIC), (300, 264, 4112, None),
+    (100, 8192, 4112, None), (300, 264, 4112, None),
+    # a short K that ends inside a K block: one block, the first of two, the fourth
+    (65, 24, 48, TILE64), (130, 200, 400, TILES), (1000, 8304, 16, TILES), (65, 1000, 112, TILE64), (257, 520, 144, TILES), (300, 4096, 496, TILES),
+    (2000, 3000, 64, TILES), (4096, 264, 272, TILES),
 ]
 
 
@@ -45,12 +49,15 @@ def test_product(dev, m, n, k, kernel, dtype, with_bias):
     out = int8_scaled_mm_azp(a, w.t(), sa, sb, dtype, zp, sums, bias)
     ran = lib.sglamd_last_gemm_kernel()
     rl.check_product(out, a, zp, w, sa, sb, bias)
-    # without zero points it is the symmetric product, on the same kernel, to the bit
+    # without zero points it is the symmetric product, on the same kernel to the bit (a short ragged K has another one there)
     none = int8_scaled_mm_azp(a, w.t(), sa, sb, dtype, torch.zeros_like(zp), sums, bias)
-    assert torch.equal(none, int8_scaled_mm(a, w.t(), sa, sb, dtype, bias))
-    assert ran == lib.sglamd_last_gemm_kernel()
+    rl.check_product(none, a, None, w, sa, sb, bias)
+    symmetric = int8_scaled_mm(a, w.t(), sa, sb, dtype, bias)
+    assert ran == lib.sglamd_last_gemm_kernel() or (k < 512 and k % 128)
+    if ran == lib.sglamd_last_gemm_kernel():
+        assert torch.equal(none, symmetric)
     if kernel is not None:
-        assert ran == kernel, f"ran kernel {ran}, meant for {kernel}"
+        assert ran in (kernel if isinstance(kernel, tuple) else (kernel,)), f"ran kernel {ran}, meant for {kernel}"
     # in the same bits on every run
     assert torch.equal(out, int8_scaled_mm_azp(a, w.t(), sa, sb, dtype, zp, sums, bias))
 
@@ -67,7 +74,23 @@ def test_all_kernels_are_among_the_sizes(dev):
         out = int8_scaled_mm_azp(a, w.t(), s[:m], s[:n], torch.bfloat16, i[:m], i[:n])
         assert not out.any()
         ran.add(lib.sglamd_last_gemm_kernel())
-    assert ran >= {STREAMING, TILE64, TILE128, TILE256, GENERIC, TILE192, STRIP}, ran
+    assert ran >= {STREAMING, TILE64, TILE128, TILE256, TILE192, STRIP}, ran
+
+
+@pytest.mark.parametrize("k", [48, 528])
+def test_rows_further_apart_than_32_bits_reach(dev, k):
+    """The generic kernel, which alone addresses operands beyond 2 GiB: 70 rows of them, 32 MB apart."""
+    from sglang_amd import int8_scaled_mm_azp
+    from sglang_amd._lib import lib
+    from sglang_amd.quantization.int8_utils import int8_weight_sums
+
+    _, w, zp, sa, sb, _ = _operands(dev, 70, 136, k, k)
+    a = torch.randint(-128, 128, (70, k), dtype=torch.int8, device=dev)
+    far = torch.empty(70 << 25, dtype=torch.int8, device=dev).as_strided((70, k), (1 << 25, 1)).copy_(a)
+    sums = int8_weight_sums(w.t())
+    out = int8_scaled_mm_azp(far, w.t(), sa, sb, torch.bfloat16, zp, sums)
+    assert lib.sglamd_last_gemm_kernel() == GENERIC
+    assert torch.equal(out, int8_scaled_mm_azp(a, w.t(), sa, sb, torch.bfloat16, zp, sums))
 
 
 def test_the_largest_sums(dev):
