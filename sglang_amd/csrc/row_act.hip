@@ -61,7 +61,7 @@ extern "C" int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_str
   hipStream_t st = (hipStream_t)stream;
   if (dtype == SGLAMD_BF16) launch_row_out<BF16, F32, ROW_PLAIN, ROW_TO_ASYM>(a, row_out_pieces(a), st);
   else if (dtype == SGLAMD_F16) launch_row_out<F16, F32, ROW_PLAIN, ROW_TO_ASYM>(a, row_out_pieces(a), st);
-  else launch_row_out<F32, F32, ROW_PLAIN, ROW_TO_ASYM>(a, false, st);
+  else launch_row_out<F32, F32, ROW_PLAIN, ROW_TO_ASYM>(a, ROW_VALUES, st);
   return check_launch(op);
 }
 

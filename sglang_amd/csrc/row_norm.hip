@@ -4,7 +4,7 @@
 using namespace sglamd;
 
 template <typename T>
-static int rms_to(const RowOutArgs& a, int weight_dtype, int q_kind, bool pieces, hipStream_t st) {
+static int rms_to(const RowOutArgs& a, int weight_dtype, int q_kind, RowPieces pieces, hipStream_t st) {
   if (weight_dtype == SGLAMD_F32) return launch_row_out_to<T, F32, ROW_RMS>(a, q_kind, pieces, st);
   return launch_row_out_to<T, T, ROW_RMS>(a, q_kind, pieces, st);
 }

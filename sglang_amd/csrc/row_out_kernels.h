@@ -23,11 +23,28 @@ __device__ __forceinline__ float silu_mul(float gate, float up) {
   return gate * __builtin_amdgcn_rcpf(1.0f + t) * up;
 }
 
-// A row's lanes: TEAM = 64, one wave (no barrier), or 0, the workgroup.  Each holds NV pieces of 8 values.
-template <typename T, typename WT, int SRC, int QK, int NV, int TEAM>
+// A piece of a row in one instruction, wherever it starts (global memory takes any alignment).
+template <typename V, bool RAGGED, typename E>
+__device__ __forceinline__ V load_piece(const E* p) {
+  if constexpr (!RAGGED) return *(const V*)p;
+  V v;
+  __builtin_memcpy(&v, p, sizeof(V));
+  return v;
+}
+template <bool RAGGED, typename V, typename E>
+__device__ __forceinline__ void store_piece(E* p, const V& v) {
+  if constexpr (RAGGED) __builtin_memcpy(p, &v, sizeof(V));
+  else *(V*)p = v;
+}
+
+// A row's lanes: TEAM = 64, one wave (no barrier), or 0, the workgroup.  Each holds NV pieces of 8 values.  RAGGED: rows of any
+// alignment and any length from 8; the last piece is the row's last 8 values, of which those that the piece before it has too
+// are written twice and counted once.
+template <typename T, typename WT, int SRC, int QK, int NV, int TEAM, bool RAGGED>
 __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t row, uint32_t* red) {
   const int nt = TEAM ? TEAM : (int)blockDim.x, tid = TEAM ? (int)threadIdx.x & 63 : (int)threadIdx.x;
-  const int nvec = row < a.rows ? (int)(a.hidden >> 3) : 0;
+  const int hidden = (int)a.hidden, nvec = row < a.rows ? (RAGGED ? (hidden + 7) >> 3 : hidden >> 3) : 0;
+  auto start = [&](int i) { return RAGGED ? min(i * 8, hidden - 8) : i * 8; };
   const u16* x = (const u16*)a.x + row * a.x_stride;
   const v4i zero = {0, 0, 0, 0};
 
@@ -37,15 +54,15 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
   for (int k = 0; k < NV; k++) {
     const int i = tid + k * nt;
     const bool live = i < nvec;
-    raw[k] = live ? *((const v4i*)x + i) : zero;
-    if constexpr (SRC == ROW_SILU) second[k] = live ? *((const v4i*)(x + a.hidden) + i) : zero;
+    raw[k] = live ? load_piece<v4i, RAGGED>(x + start(i)) : zero;
+    if constexpr (SRC == ROW_SILU) second[k] = live ? load_piece<v4i, RAGGED>(x + hidden + start(i)) : zero;
     if constexpr (SRC == ROW_RMS) {
-      second[k] = live && a.res ? *((const v4i*)((const u16*)a.res + row * a.res_stride) + i) : zero;
+      second[k] = live && a.res ? load_piece<v4i, RAGGED>((const u16*)a.res + row * a.res_stride + start(i)) : zero;
       if constexpr (sizeof(typename WT::storage) == 4) {
-        wraw[k][0] = live ? *((const v4i*)a.w + 2 * i) : zero;
-        wraw[k][1] = live ? *((const v4i*)a.w + 2 * i + 1) : zero;
+        wraw[k][0] = live ? load_piece<v4i, RAGGED>((const float*)a.w + start(i)) : zero;
+        wraw[k][1] = live ? load_piece<v4i, RAGGED>((const float*)a.w + start(i) + 4) : zero;
       } else {
-        wraw[k][0] = live ? *((const v4i*)a.w + i) : zero;
+        wraw[k][0] = live ? load_piece<v4i, RAGGED>((const u16*)a.w + start(i)) : zero;
       }
     }
   }
@@ -69,7 +86,7 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
 #pragma unroll
         for (int j = 0; j < 8; j++) u[k][j] += r[j];
         const int i = tid + k * nt;
-        if (i < nvec) *((v4i*)((u16*)a.res_out + row * a.hidden) + i) = pack8<T>(u[k]);
+        if (i < nvec) store_piece<RAGGED>((u16*)a.res_out + row * a.hidden + start(i), pack8<T>(u[k]));
       }
       float w[8];
       if constexpr (sizeof(typename WT::storage) == 4) {
@@ -79,7 +96,8 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        t.ss = fmaf(u[k][j], u[k][j], t.ss);
+        const int i = tid + k * nt;
+        if (!RAGGED || start(i) + j >= i * 8) t.ss = fmaf(u[k][j], u[k][j], t.ss);
         u[k][j] *= w[j];
       }
     }
@@ -102,12 +120,12 @@ __device__ __forceinline__ void row_out_body(const RowOutArgs& a, const int64_t 
   for (int k = 0; k < NV; k++) {
     const int i = tid + k * nt;
     if (i >= nvec) break;
-    *((v2i*)q + i) = v2i{(int)row_codes4<QK>(u[k], o), (int)row_codes4<QK>(u[k] + 4, o)};
+    store_piece<RAGGED>(q + start(i), v2i{(int)row_codes4<QK>(u[k], o), (int)row_codes4<QK>(u[k] + 4, o)});
     if (SRC == ROW_RMS && a.y) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] = u[k][j] * o.r;
-      *((v4i*)((u16*)a.y + row * a.hidden) + i) = pack8<T>(y);
+      store_piece<RAGGED>((u16*)a.y + row * a.hidden + start(i), pack8<T>(y));
     }
   }
 }
@@ -120,18 +138,18 @@ static inline dim3 row_out_grid(int64_t blocks) {
   return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)ceil_div(blocks, most));
 }
 
-template <typename T, typename WT, int SRC, int QK, int NT, int NV>
+template <typename T, typename WT, int SRC, int QK, int NT, int NV, bool RAGGED>
 __global__ __launch_bounds__(NT) void row_out_kernel(RowOutArgs a) {
   __shared__ uint32_t red[48];
-  row_out_body<T, WT, SRC, QK, NV, 0>(a, row_out_block(), red);
+  row_out_body<T, WT, SRC, QK, NV, 0, RAGGED>(a, row_out_block(), red);
 }
 // Short rows, a wave each.
-template <typename T, typename WT, int SRC, int QK, int NV>
+template <typename T, typename WT, int SRC, int QK, int NV, bool RAGGED>
 __global__ __launch_bounds__(256) void row_out_team_kernel(RowOutArgs a) {
-  row_out_body<T, WT, SRC, QK, NV, 64>(a, row_out_block() * 4 + (threadIdx.x >> 6), nullptr);
+  row_out_body<T, WT, SRC, QK, NV, 64, RAGGED>(a, row_out_block() * 4 + (threadIdx.x >> 6), nullptr);
 }
 
-// Any row length and alignment, 32-bit rows: a workgroup per row, values one by one, the row read twice (the second time
+// Rows below 8 values and beyond 32768, 32-bit rows: a workgroup per row, values one by one, the row read twice (the second time
 // from L2).
 template <typename T, typename WT, int SRC, int QK>
 __global__ __launch_bounds__(256) void row_out_any_kernel(RowOutArgs a) {
@@ -187,19 +205,15 @@ constexpr int64_t ROW_OUT_MAX_HIDDEN = 512 * 8 * 8;  // the longest row that 512
 //   1024 x 2                 norm 4096 x 14336 77 | 78 (512 x 4), SiLU 54.6 | 56.7, plain 33.9 | 34.1
 //   512 x 8                  SiLU 3001 x 18432 53.8 | 55.0 (1024 x 4), 2000 x 28672 54.4 | 56.6
 //   1024 x 4                 norm 4096 x 18432 114.9 | 118.5 (512 x 8), SiLU to symmetric codes, which keep fewer registers, 72.8 | 76.0
-template <typename T, typename WT, int SRC, int QK>
-static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
-  const dim3 grid = row_out_grid(a.rows);
-  if (!pieces) {
-    hipLaunchKernelGGL((row_out_any_kernel<T, WT, SRC, QK>), grid, dim3(256), 0, st, a);
-    return;
-  }
+template <typename T, typename WT, int SRC, int QK, bool RAGGED>
+static void launch_row_pieces(const RowOutArgs& a, hipStream_t st) {
   if constexpr (sizeof(typename T::storage) == 2) {
-    const int64_t nvec = a.hidden >> 3;
+    const dim3 grid = row_out_grid(a.rows);
+    const int64_t nvec = (a.hidden + 7) >> 3;
     const bool many = a.rows >= 2 * (int64_t)device_cus();
     constexpr bool RMS = SRC == ROW_RMS, PLAIN = SRC == ROW_PLAIN;
-#define SGLAMD_ROW_TEAM(NV) hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, NV>), row_out_grid(ceil_div(a.rows, 4)), dim3(256), 0, st, a)
-#define SGLAMD_ROW_OUT(NT, NV) hipLaunchKernelGGL((row_out_kernel<T, WT, SRC, QK, NT, NV>), grid, dim3(NT), 0, st, a)
+#define SGLAMD_ROW_TEAM(NV) hipLaunchKernelGGL((row_out_team_kernel<T, WT, SRC, QK, NV, RAGGED>), row_out_grid(ceil_div(a.rows, 4)), dim3(256), 0, st, a)
+#define SGLAMD_ROW_OUT(NT, NV) hipLaunchKernelGGL((row_out_kernel<T, WT, SRC, QK, NT, NV, RAGGED>), grid, dim3(NT), 0, st, a)
     if (nvec <= 64) SGLAMD_ROW_TEAM(1);
     else if (nvec <= 128 && (many || !RMS)) SGLAMD_ROW_TEAM(2);
     else if (PLAIN && many && nvec <= 256) SGLAMD_ROW_TEAM(PLAIN ? 4 : 2);
@@ -212,8 +226,18 @@ static void launch_row_out(const RowOutArgs& a, bool pieces, hipStream_t st) {
 #undef SGLAMD_ROW_TEAM
   }
 }
+// How the rows can be taken: in pieces of 8 values, 16 bytes in and 8 out, that stay in registers, each of them aligned or not, or
+// value by value.  Aligned | unaligned, us: norm 4096 x 8192 39.8 | 43.8, SiLU 30.4 | 33.9, norm of one row of 7168 3.2 | 4.0.  Unaligned |
+// value by value: norm 4096 x 4095 22.4 | 58.9, SiLU 892 x 10542 13.3 | 41.9, norm of one row of 7169 3.3 | 18.9.
+enum RowPieces { ROW_VALUES, ROW_PIECES_ANYWHERE, ROW_PIECES };
+template <typename T, typename WT, int SRC, int QK>
+static void launch_row_out(const RowOutArgs& a, RowPieces pieces, hipStream_t st) {
+  if (pieces == ROW_PIECES) launch_row_pieces<T, WT, SRC, QK, false>(a, st);
+  else if (pieces == ROW_PIECES_ANYWHERE) launch_row_pieces<T, WT, SRC, QK, true>(a, st);
+  else hipLaunchKernelGGL((row_out_any_kernel<T, WT, SRC, QK>), row_out_grid(a.rows), dim3(256), 0, st, a);
+}
 template <typename T, typename WT, int SRC>
-static int launch_row_out_to(const RowOutArgs& a, int q_kind, bool pieces, hipStream_t st) {
+static int launch_row_out_to(const RowOutArgs& a, int q_kind, RowPieces pieces, hipStream_t st) {
   if (q_kind == ROW_TO_FP8) launch_row_out<T, WT, SRC, ROW_TO_FP8>(a, pieces, st);
   else if (q_kind == ROW_TO_INT8) launch_row_out<T, WT, SRC, ROW_TO_INT8>(a, pieces, st);
   else launch_row_out<T, WT, SRC, ROW_TO_ASYM>(a, pieces, st);
@@ -236,11 +260,12 @@ static inline int row_out_kind(const RowOutArgs& a, int q_dtype) {
   return q_dtype == SGLAMD_FP8_E4M3 ? ROW_TO_FP8 : a.zp ? ROW_TO_ASYM : ROW_TO_INT8;
 }
 static inline bool aligned_to(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
-// Whether the rows can be taken in pieces of 8 values, 16 bytes in and 8 out, and kept in registers.
-static inline bool row_out_pieces(const RowOutArgs& a) {
-  return a.hidden % 8 == 0 && a.hidden <= ROW_OUT_MAX_HIDDEN && a.x_stride % 8 == 0 && aligned_to(a.x, 16) && aligned_to(a.q, 8) &&
-         (!a.res || (a.res_stride % 8 == 0 && aligned_to(a.res, 16) && aligned_to(a.res_out, 16))) && (!a.w || aligned_to(a.w, 16)) &&
-         (!a.y || aligned_to(a.y, 16));
+static inline RowPieces row_out_pieces(const RowOutArgs& a) {
+  if (a.hidden < 8 || a.hidden > ROW_OUT_MAX_HIDDEN) return ROW_VALUES;
+  const bool aligned = a.hidden % 8 == 0 && a.x_stride % 8 == 0 && aligned_to(a.x, 16) && aligned_to(a.q, 8) &&
+                       (!a.res || (a.res_stride % 8 == 0 && aligned_to(a.res, 16) && aligned_to(a.res_out, 16))) && (!a.w || aligned_to(a.w, 16)) &&
+                       (!a.y || aligned_to(a.y, 16));
+  return aligned ? ROW_PIECES : ROW_PIECES_ANYWHERE;
 }
 
 }  // namespace sglamd

@@ -12,7 +12,8 @@ With y the row before its codes, all in float32 and not rounded on the way:
 
 The codes are (q, scale) or (q, scale, zp): q like the row, scale float32 [M, 1], zp int32 [M, 1]; y is about
 scale * (q - zp).  A row of y that holds a NaN or an infinity gets a scale that is NaN or infinite; with a given scale a NaN stays
-a NaN code and an infinity saturates (behind the norm the whole row is NaN).  Rows may have any length and stride; multiples of 8 in 16-byte aligned rows are the fast ones.  There is no gradient."""
+a NaN code and an infinity saturates (behind the norm the whole row is NaN).  Rows may have any length, alignment and stride; those of 8 to 32768 values are
+read once.  There is no gradient."""
 from typing import Optional, Tuple
 
 import torch

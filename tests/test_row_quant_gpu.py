@@ -23,9 +23,11 @@ def _rows(g, *shape, dtype=torch.bfloat16, shift=0.0):
     return (torch.randn(*shape, generator=g) * 2 + shift).to(dtype)
 
 
-# (teams of a wave, one workgroup form after the other, the value-by-value form: odd lengths and rows beyond 32768)
+# (teams of a wave, one workgroup form after the other, each with pieces that are aligned and with pieces that overlap at the end, the
+# value-by-value form: fewer than 8 values and more than 32768)
 ROW_SIZES = [(1, 1), (3, 7), (2, 8), (5, 24), (1, 128), (700, 512), (600, 1000), (40, 1000), (600, 2000), (37, 1536), (1, 7168), (530, 4096), (515, 8192),
-             (7, 8184), (9, 16384), (3, 28672), (2, 32776), (4, 4099)]
+             (7, 8184), (9, 16384), (3, 28672), (2, 32776), (4, 4099), (3, 9), (5, 15), (700, 513), (600, 1001), (40, 1023), (600, 2046), (37, 1537), (530, 4095),
+             (515, 8191), (9, 16383), (3, 28673), (2, 32767)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
