@@ -3,7 +3,11 @@
 In a decode step the norm in front of the experts hands over codes and scales (quantization.fused_row_quant) beside the 16-bit
 row that the router reads, so the layer has nothing to quantise or sort in front of its first product: pairs that share an
 expert are found inside the kernels, and the sum over a token's experts ends the second one.  The general layer
-(fused_experts; python/sglang/srt/layers/moe/moe_runner/triton_utils/fused_moe.py:401-785) takes 16-bit rows and any number of them."""
+(fused_experts; python/sglang/srt/layers/moe/moe_runner/triton_utils/fused_moe.py:401-785) takes 16-bit rows and any number of them.
+
+Which of the two: this one reads an expert's weights once for every four rows that meet it, the general one once.  Int8, us, quantiser
+included, here | fused_experts: 128 experts of 2048 x 768, 8 each, 1 / 4 / 8 tokens 15 | 30, 36 | 47, 56 | 66; 64 of 4096 x 1536, 8 each, 1 / 8
+34 | 49, 133 | 140; but 8 of 4096 x 1536, 2 each, 8 / 16 / 32 tokens 37 | 43, 52 | 49, 87 | 50."""
 from typing import Optional
 
 import torch

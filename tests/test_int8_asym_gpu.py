@@ -243,3 +243,30 @@ def test_refusals(dev):
         apply_int8_linear(x.float(), w.t(), sb)
     with pytest.raises(NotImplementedError):
         apply_int8_linear(x.requires_grad_(), w.t(), sb)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (5, 520, 2048), (40, 8192, 4096), (300, 512, 8192), (300, 1024, 336)])
+@pytest.mark.parametrize("asym", [False, True])
+def test_linear_captured_and_replayed(dev, m, n, k, asym):
+    """Rows quantised in the product, by a launch in front, K in slices: captured once, replayed on changing rows between eager calls."""
+    from sglang_amd.quantization.int8_utils import apply_int8_linear, int8_weight_sums
+
+    _, w, _, _, sb, bias = _operands(dev, 1, n, k, m)
+    sums, bias = int8_weight_sums(w.t()) if asym else None, bias.bfloat16()
+    g = torch.Generator().manual_seed(m)
+    inputs = [torch.randn(m, k, generator=g).to(torch.bfloat16).to(dev) for _ in range(3)]
+    x = inputs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        apply_int8_linear(x, w.t(), sb, sums, bias=bias)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = apply_int8_linear(x, w.t(), sb, sums, bias=bias)
+    for i in range(6):
+        want = apply_int8_linear(inputs[i % 3], w.t(), sb, sums, bias=bias)
+        x.copy_(inputs[i % 3])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
