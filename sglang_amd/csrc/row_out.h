@@ -156,8 +156,9 @@ __device__ __forceinline__ RowScale row_scale(const RowOutArgs& a, const RowStat
     o.scale = amax / 127.0f;
     o.mul = o.r * (127.0f / amax);
   } else {
-    const float lo = __uint_as_float(t.lo) * o.r, span = hi + lo;
-    o.scale = (span > 1e-10f || span != span ? span : 1e-10f) / 255.0f;
+    // (half the span: that of finite values may be beyond fp32; halves round as the whole does)
+    const float lo = __uint_as_float(t.lo) * o.r, half = 0.5f * hi + 0.5f * lo;
+    o.scale = (half > 0.5e-10f || half != half ? half : 0.5e-10f) / 127.5f;
     o.mul = o.r / o.scale;
     o.zp = __builtin_amdgcn_fmed3f(rintf(-128.0f + lo / o.scale), -128.f, 127.f);
   }
