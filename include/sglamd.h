@@ -493,8 +493,8 @@ int sglamd_per_token_quant_int8_asym(const void* x, int64_t x_row_stride, int dt
  * w13_scale fp32 [E, 2 * I], w2_scale [E, H]; b13, b2 optional, shaped like the scales, in out_dtype (F16/BF16);
  * topk_weights fp32 [M, topk], topk_ids [M, topk] int32 or int64: pairs whose id is outside [0, E) contribute nothing, an
  * id may be named more than once.  H and I multiples of 16, H <= 32768, I <= 16384, M * topk <= 64 (more: SGLAMD_ENOTSUP).  workspace:
- * sglamd_fused_experts_few_tokens_workspace(...) bytes, 16-byte aligned, nothing in it has to start at zero; calls that
- * overlap need workspaces of their own. */
+ * sglamd_fused_experts_few_tokens_workspace(...) bytes (0 for sizes that the layer refuses), 16-byte aligned, nothing in it has to
+ * start at zero; calls that overlap need workspaces of their own. */
 int64_t sglamd_fused_experts_few_tokens_workspace(int64_t M, int64_t I, int topk);
 int sglamd_fused_experts_few_tokens(const void* x, const float* x_scale, int q_dtype, int64_t M, int64_t H, int64_t I,
                                     int E, int topk, const void* w13, const float* w13_scale, const void* b13,

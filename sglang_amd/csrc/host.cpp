@@ -1306,16 +1306,20 @@ Tensor experts_few_tokens(const Tensor& x, const Tensor& xs, const Tensor& w1, c
   check_same_device(weights, x, "topk_weights");
   const int64_t topk = ids.size(1);
   const c10::DeviceGuard guard(x.device());
-  Tensor out = empty({m, h}, out_dtype, x);
-  if (m == 0) return out;
+  if (m == 0) return empty({m, h}, out_dtype, x);
   const Tensor tw = weights.to(at::kFloat).contiguous(), at_ids = ids.contiguous();
   const int64_t need = sglamd_fused_experts_few_tokens_workspace(m, i, (int)std::min<int64_t>(topk, 1 << 20));
-  const Tensor ws = empty({std::max<int64_t>(need, 16)}, at::kByte, x);
-  check(sglamd_fused_experts_few_tokens(x.data_ptr(), xs.data_ptr<float>(), tag(qt), m, h, i, (int)std::min<int64_t>(e, 0x7fffffff),
-                                        (int)std::min<int64_t>(topk, 1 << 20), w1.data_ptr(), s1.data_ptr<float>(), b1 ? b1->data_ptr() : nullptr,
-                                        w2.data_ptr(), s2.data_ptr<float>(), b2 ? b2->data_ptr() : nullptr, tw.data_ptr<float>(),
-                                        at_ids.data_ptr(), tag(at_ids.scalar_type()), out.data_ptr(), tag(out_dtype), (float)factor, ws.data_ptr(),
-                                        need, stream_of(x)));
+  auto run = [&](void* out, void* workspace) {
+    check(sglamd_fused_experts_few_tokens(x.data_ptr(), xs.data_ptr<float>(), tag(qt), m, h, i, (int)std::min<int64_t>(e, 0x7fffffff),
+                                          (int)std::min<int64_t>(topk, 1 << 20), w1.data_ptr(), s1.data_ptr<float>(), b1 ? b1->data_ptr() : nullptr,
+                                          w2.data_ptr(), s2.data_ptr<float>(), b2 ? b2->data_ptr() : nullptr, tw.data_ptr<float>(),
+                                          at_ids.data_ptr(), tag(at_ids.scalar_type()), out, tag(out_dtype), (float)factor, workspace, need,
+                                          stream_of(x)));
+  };
+  if (need == 0) run(x.data_ptr(), x.data_ptr());  // (no workspace: sizes that the layer refuses, here in front of the allocations)
+  Tensor out = empty({m, h}, out_dtype, x);
+  const Tensor ws = empty({need}, at::kByte, x);
+  run(out.data_ptr(), ws.data_ptr());
   return out;
 }
 

@@ -472,7 +472,8 @@ static int few_layer(const FewArgs& up, const FewArgs& down, hipStream_t st) {
 using namespace sglamd;
 
 extern "C" int64_t sglamd_fused_experts_few_tokens_workspace(int64_t M, int64_t I, int topk) {
-  return M > 0 && I > 0 && topk > 0 && M <= FEW_MAX_PAIRS && topk <= FEW_MAX_PAIRS && I <= FEW_MAX_INTER ? M * topk * I * 4 : 0;
+  const bool taken = M > 0 && I > 0 && topk > 0 && M <= FEW_MAX_PAIRS && topk <= FEW_MAX_PAIRS && M * topk <= FEW_MAX_PAIRS && I <= FEW_MAX_INTER;
+  return taken ? M * topk * I * 4 : 0;
 }
 
 extern "C" int sglamd_fused_experts_few_tokens(const void* x, const float* x_scale, int q_dtype, int64_t M, int64_t H, int64_t I, int E, int topk,
