@@ -99,7 +99,7 @@ int sglamd_tensor_absmax_scale(const void* input, int in_dtype, int64_t numel, f
                                float* workspace, void* stream);
 
 /* Per-token symmetric INT8 quantisation: amax = max(max|x|, 1e-10), scale = amax/127,
- * q = int8(round_half_away_from_zero(x * (127/amax))).
+ * q = int8(round_half_away_from_zero(x * (127/amax))).  The maximum skips a NaN, whose code is 0.
  * Stands in for the Triton per_token_quant_int8
  * (python/sglang/srt/layers/quantization/int8_kernel.py:28-89). */
 int sglamd_per_token_quant_int8(const void* input, int in_dtype, int8_t* output_q, float* output_s, int64_t rows,
@@ -235,7 +235,8 @@ int sglamd_int8_scaled_mm_azp(const void* a, int64_t lda, const void* b, int64_t
  * elements apart) quantised per token, then the product in dtype.  Without weight_sums the arithmetic of
  * sglamd_per_token_quant_int8 and sglamd_int8_scaled_mm (contiguous 16-byte aligned rows), with them that of
  * sglamd_per_token_quant_int8_asym and sglamd_int8_scaled_mm_azp; the same bits either way, in one launch where a few short rows are
- * quantised by the product's own workgroups (M <= 16, K % 128 == 0).  q int8 [M, K], sa fp32 [M] and zp int32 [M] (NULL without
+ * quantised by the product's own workgroups (M <= 16, K % 128 == 0).  A NaN in a row makes the output row NaN with weight_sums and
+ * counts as a zero without; an infinity leaves no finite value in its row either way.  q int8 [M, K], sa fp32 [M] and zp int32 [M] (NULL without
  * weight_sums) are scratch; workspace as for the products. */
 int sglamd_int8_row_linear(const void* x, int64_t x_row_stride, int dtype, int64_t M, int64_t K, const void* w,
                            int64_t ldb, const float* sb, const int32_t* weight_sums, const void* bias, void* out,

@@ -9,7 +9,8 @@ from .fp8_kernel import sglang_per_token_group_quant_int8
 
 
 def per_token_quant_int8(x: torch.Tensor, scale_dtype=torch.float32, cal_sum: bool = False):
-    """Returns (x_q int8 like x, scales [..., 1]); cal_sum additionally returns the row sums."""
+    """Returns (x_q int8 like x, scales [..., 1]); cal_sum additionally returns the row sums.  The maximum skips a NaN, whose
+    code is 0; an infinity makes its row's scale infinite."""
     assert x.is_contiguous()
     assert scale_dtype == torch.float32, "only fp32 scales are produced"
     quantised = _C.per_token_quant(x, True) if eager(x) else None

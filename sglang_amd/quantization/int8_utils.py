@@ -33,7 +33,11 @@ def apply_int8_linear(
     and without where not; the output has its dtype.  An int8 input is taken as quantised already (fused_rms_row_quant,
     silu_and_mul_row_quant, per_token_quant_int8 or per_token_quant_int8_asym): input_scale holds a value per token,
     input_zero_point too or None, and out_dtype says what the output is (bfloat16).  K % 16 == 0, N % 8 == 0; K <= 65536 with
-    zero points."""
+    zero points.
+
+    Rows that are not finite: with zero points a NaN or an infinity makes its whole output row NaN.  Without them the rows are
+    quantised as per_token_quant_int8 does it, whose maximum skips a NaN: it counts as a zero and the output does not show it,
+    while an infinity leaves no finite value in its output row.  (fused_rms_row_quant and silu_and_mul_row_quant show both in either form.)"""
     n = weight.shape[1]
     w_scale = weight_scale
     if w_scale.numel() == 1 and n != 1:
