@@ -461,7 +461,7 @@ int sglamd_fused_rms_fp8_group_quant(const void* x1, int64_t x1_row_stride, cons
  *   I8 with output_zp:  lo = min(0, min y), hi = max(0, max y), scale = max(hi - lo, 1e-10) / 255,
  *              zp = rint(-128 - lo / scale);  code = clamp(rint(y * (1 / scale)) + zp, -128, 127);  y is scale * (code - zp)
  * output_q [rows, hidden], output_s fp32 [rows] (a fixed scale is repeated), output_zp int32 [rows] or NULL.  Rows may have
- * any length, stride (in elements, 0 included) and alignment; rows of 8 to 32768 values of 16 bits are read once, in 16-byte
+ * any length and alignment, and any stride (in elements) from their length up, or 0; rows of 8 to 32768 values of 16 bits are read once, in 16-byte
  * pieces, all others value by value, twice.  Outputs overlap no input.  A row of y that
  * holds a NaN or an infinity gets a scale that is NaN or infinite, so that it stays visible behind the product.  With a fixed
  * scale a NaN is e4m3's NaN and an infinity saturates; a row whose sum of squares is not finite is all NaN.  e4m3 rows whose

@@ -12,8 +12,9 @@ With y the row before its codes, all in float32 and not rounded on the way:
 
 The codes are (q, scale) or (q, scale, zp): q like the row, scale float32 [M, 1], zp int32 [M, 1]; y is about
 scale * (q - zp).  A row of y that holds a NaN or an infinity gets a scale that is NaN or infinite; with a given scale a NaN stays
-a NaN code and an infinity saturates (behind the norm the whole row is NaN).  Rows may have any length, alignment and stride; those of 8 to 32768 values are
-read once.  There is no gradient."""
+a NaN code and an infinity saturates (behind the norm the whole row is NaN).  Rows may have any length and alignment and lie any distance apart, or be one row
+repeated (a stride of 0); rows that overlap otherwise raise.  Those of 8 to 32768 values are read once.  There is no gradient and
+no torch.ops schema: under a tracer or a transform the functions raise NotImplementedError."""
 from typing import Optional, Tuple
 
 import torch
@@ -50,5 +51,5 @@ def silu_and_mul_row_quant(
     scale: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, ...]:
     """The codes of silu(gate) * up for rows of [gate | up], input [M, 2 * N] half/bfloat16 with contiguous rows: silu_and_mul
-    and a per-token quantiser in one pass, without the rounding to 16 bits between them."""
+    and a per-token quantiser in one pass, without the rounding to 16 bits between them.  Gates below -87 give 0."""
     return _codes(*_C.silu_mul_row_quant(input, dtype_quant, symmetric, scale))

@@ -28,7 +28,7 @@ def per_token_quant_int8(x: torch.Tensor, scale_dtype=torch.float32, cal_sum: bo
 def per_token_quant_int8_asym(x: torch.Tensor):
     """(x_q int8 like x, scales float32 [..., 1], zero points int32 [..., 1]) with x about scale * (x_q - zp): the whole int8
     range over [min(0, min x), max(0, max x)] of each row (the formulas are those of fused_row_quant).  x float32, half or
-    bfloat16 [..., hidden]; 2D inputs may have any row stride."""
+    bfloat16 [..., hidden], contiguous, or 2D with rows any distance apart or one row repeated."""
     if x.dim() != 2:
         assert x.is_contiguous()
     q, s, zp = _C.per_token_quant_int8_asym(x if x.dim() == 2 else x.view(-1, x.shape[-1]))
