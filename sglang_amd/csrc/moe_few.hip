@@ -16,10 +16,12 @@
 //     the rows of its group itself, in front of which it has requested its first weights; the pairs' results meet in LDS and
 //     are summed in the pairs' order, so the sum over a token's experts needs neither atomics nor a launch.
 //
-// Measured (kernels, us; in brackets a bare read of the weights' bytes): 6 of 64 int8 experts of 4096 x 1536, one token, 15.2 + 10.6
-// (16.4); 8 of 128 e4m3 experts of 2048 x 768, three tokens, 15.1 + 11.0 (15.5); 8 of 256 of 7168 x 2048, one token 38.7 + 23.2 (51),
-// four 133 + 80 (195).  Large layers run at the rate of a read; small ones wait for two launches, and in each for a chain of ids, rows
-// and first weights, some 4 us a launch.
+// Measured (medians of traced launches, us; in brackets a bare read of the weights' bytes): 6 of 64 int8 experts of 4096 x 1536, one token,
+// 14.1 + 10.3 (16.4); 8 of 128 e4m3 experts of 2048 x 768, three tokens, 14.6 + 11.5 (15.5); 8 of 256 of 7168 x 2048, one token 36.9 + 22.8
+// (51), four 130 + 79 (195).  Large layers run at the rate of a read; small ones wait for two launches, and in each for a chain of ids, rows
+// and first weights, some 4 us a launch.  Intermediate sizes beyond 2048 are far from it: the rows of a pass below, in few_layer, and too few
+// waves in the second launch (8 int8 experts of 4096 x 14336, both launches and the quantiser, a read in brackets: two pairs of one token 101
+// (51), eight tokens of two 603 (205)).
 // Tried: the second launch's rows quantised by the workgroup together, behind a barrier (four tokens of the large layer 80 -> 89: all
 // waves quantise at once and all stream at once); sixteen waves to all its workgroups (registers spill, or fewer are left for the loads:
 // four tokens of the large layer 205 -> 214, both launches); a wave's next group requested under the results of the one before
@@ -448,7 +450,8 @@ static int few_start_down(const FewArgs& a, hipStream_t st) {
 template <bool INT8, typename OT>
 static int few_layer(const FewArgs& up, const FewArgs& down, hipStream_t st) {
   const int pairs = up.M * up.topk, cus = device_cus();
-  // Rows that one pass over an expert's weights serves: as many as there are tokens, as LDS holds of them.
+  // Rows that one pass over an expert's weights serves, in both launches: as many as there are tokens, as LDS holds of them (with eight pairs
+  // and more four up to I = 2048, two up to 4096, else one).
   int rmax = up.M == 1 ? 1 : up.M == 2 ? 2 : 4;
   while (rmax > 1 && (std::min(pairs, FEW_DOWN_WAVES) * rmax * up.I > FEW_LDS || rmax * up.H > FEW_LDS)) rmax /= 2;
   // Lanes per weight row.  First launch: eight, where that gives a CU six waves, else 32 (8 | 32 lanes: 7168 x 2048, one token, eight waves

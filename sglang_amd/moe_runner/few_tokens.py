@@ -5,9 +5,13 @@ row that the router reads, so the layer has nothing to quantise or sort in front
 expert are found inside the kernels, and the sum over a token's experts ends the second one.  The general layer
 (fused_experts; python/sglang/srt/layers/moe/moe_runner/triton_utils/fused_moe.py:401-785) takes 16-bit rows and any number of them.
 
-Which of the two: this one reads an expert's weights once for every four rows that meet it, the general one once.  Int8, us, quantiser
-included, here | fused_experts: 128 experts of 2048 x 768, 8 each, 1 / 4 / 8 tokens 15 | 30, 36 | 47, 56 | 66; 64 of 4096 x 1536, 8 each, 1 / 8
-34 | 49, 133 | 140; but 8 of 4096 x 1536, 2 each, 8 / 16 / 32 tokens 37 | 43, 52 | 49, 87 | 50."""
+Which of the two: the general one reads an expert's weights once; this one once for every pass over the rows that meet it, of one row at one
+token, two at two, else four, and fewer where eight waves' rows of I codes do not fit 64 KB (from eight pairs on two beyond I = 2048, one beyond
+4096) or sixteen waves share the second launch (two).  Int8, us, quantiser included, here | fused_experts: 128 experts of 2048 x 768, 8 each,
+1 / 4 / 8 tokens 16 | 30, 33 | 49, 53 | 63; 64 of 4096 x 1536, 8 each, 1 / 4 / 8 34 | 48, 90 | 101, 149 | 160; 8 of 4096 x 1536, 2 each, 4 / 8 / 16 / 32
+26 | 37, 34 | 39, 58 | 49, 78 | 50; 16 of 4096 x 4096, 2 each, 1 / 4 / 8 / 16 34 | 40, 81 | 80, 117 | 102, 193 | 117; 8 of 4096 x 14336, 2 each,
+1 / 4 / 8 101 | 74, 275 | 185, 603 | 233.  So: this one for I up to 2048 while experts meet up to two or three rows each, up to 4096 at about
+one row each, the general one otherwise."""
 from typing import Optional
 
 import torch
@@ -18,7 +22,8 @@ MAX_PAIRS = 64
 
 
 def takes_few_tokens(num_tokens: int, topk: int) -> bool:
-    """Whether fused_experts_few_tokens takes so many tokens and experts per token."""
+    """Whether fused_experts_few_tokens takes so many tokens and experts per token (not whether it is faster than fused_experts
+    on them: the head of this file has the times)."""
     return num_tokens * topk <= MAX_PAIRS
 
 
