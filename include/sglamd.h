@@ -617,6 +617,90 @@ int sglamd_fp8_blockwise_scaled_grouped_mm(void* output, int out_dtype, const vo
                                            void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * Between a projection and its attention (no single counterpart in the reference): heads of queries, keys and values through
+ * RMSNorm, rotary positions and into a paged cache, in one launch; rows of such a cache back in 16 bits.
+ * ------------------------------------------------------------------------------------ */
+
+/* A cache of `pages` pages of `page_size` slots and the slot of every token (a gathered row: the slot that it comes from), I32 or
+ * I64, slot_stride elements apart.  Slot s is row s % page_size of page s / page_size.  A slot outside [0, pages * page_size) is
+ * none: such a token writes nothing to the cache, such a gathered row is zeros.  Slots of one launch that write have to differ:
+ * where two are the same, each 2 to 32 bytes of the row are of one of the two tokens.  pages * page_size < 2^31. */
+typedef struct {
+  const void* slots;
+  int slots_dtype;
+  int64_t slot_stride, page_size, pages;
+} sglamd_slots;
+
+/* Rotary positions.  The table has a row of width / 2 cosines and then width / 2 sines per position, table_dtype F32 or the heads'
+ * type, rows table_stride elements apart.  Pair i < width / 2 of a head is (x[i], x[i + width / 2]), interleaved: (x[2 i], x[2 i + 1]);
+ * (a, b) becomes (a cos - b sin, b cos + a sin), the values behind the first `width` stay.  The position of token t on axis k is
+ * positions[k * axis_stride + t * position_stride], I32 or I64.  With more than one axis, sections[k] pairs turn by axis k: the
+ * first sections[0] by axis 0 and so on, alternating: pair i by axis i % axes where i < axes * sections[i % axes], by axis 0
+ * otherwise.  A position outside of the table gives NaN. */
+typedef struct {
+  const void* cos_sin;
+  int table_dtype;
+  int64_t table_rows, table_stride, width;
+  int interleaved;
+  const void* positions;
+  int positions_dtype;
+  int64_t axis_stride, position_stride;
+  int axes; /* 1 to 4 */
+  int32_t sections[4];
+  int alternating;
+} sglamd_rotation;
+
+/* One tensor x of heads [tokens, heads, dim], strides in elements, dim contiguous, even, at most 1024.  In fp32, rounded once at
+ * the end:  y = x;  with a weight (F32 or the heads' type, [dim]) y = x / sqrt(mean(x^2) + eps) * weight over each head (a head
+ * whose sum of squares is not finite in fp32 is NaN);  rotate: its first rotation.width values turned.
+ *   out    optional: y in the heads' type; may be x itself
+ *   cache  optional: y in the slots' rows, strides in elements; cache_dtype the heads' type, or
+ *          FP8_E4M3: code = e4m3(clamp(y / scale, -448, 448)) with given_scale[head * given_head], or with
+ *                    scale = max|y| / 448 of each row, written to `scales`
+ *          I8:       code = round(y / scale), scale = max(max|y|, 1e-10) / 127 of each row, written to `scales`
+ *          scale_group: dim (one scale per row), or 128: one per 128 values, scales_group elements apart, for heads that are
+ *          not rotated and whose dim is a multiple of 128.  A row that holds a NaN or an infinity gets such a scale.
+ * Memory that is written overlaps nothing else that the launch reads or writes, but for out == x. */
+typedef struct {
+  const void* x;
+  int64_t x_token, x_head, heads, dim;
+  const void* weight;
+  int weight_dtype;
+  float eps;
+  int rotate;
+  void* out;
+  int64_t out_token, out_head;
+  void* cache;
+  int cache_dtype;
+  int64_t cache_page, cache_slot, cache_head;
+  const float* given_scale;
+  int64_t given_head;
+  float* scales;
+  int64_t scales_page, scales_slot, scales_head, scales_group, scale_group;
+} sglamd_heads;
+
+/* One to four tensors of heads of the same tokens and of one type (dtype F16 or BF16).  `parts`, `rotation` (NULL: nothing is
+ * rotated) and `slots` (NULL: no cache) are host structures, read before the call returns. */
+int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_t tokens, int dtype, const sglamd_rotation* rotation,
+                     const sglamd_slots* slots, void* stream);
+
+/* out[row] = the cache's row of slots[row], times its scale, in `dtype` (F16 or BF16, the cache's own type where that has 16 bits):
+ * one or two caches of the same slots, fields as in sglamd_heads; dim at most 1024. */
+typedef struct {
+  const void* cache;
+  int cache_dtype;
+  int64_t cache_page, cache_slot, cache_head, heads, dim;
+  const float* given_scale;
+  int64_t given_head;
+  const float* scales;
+  int64_t scales_page, scales_slot, scales_head, scales_group, scale_group;
+  void* out;
+  int64_t out_row, out_head;
+} sglamd_gather;
+int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts, int64_t rows, int dtype, const sglamd_slots* slots,
+                            void* stream);
+
+/* ------------------------------------------------------------------------------------
  * Measured ceilings (no counterpart in the reference; launched by the benchmark only): bare loops that show what
  * the GPU gives a kernel at best, for reading the roofline fractions against.
  * sglamd_ceiling_mfma: 256 workgroups x 8 waves, each wave `iters` rounds of 8 MFMA tiles 32x32x64 (FP8:

@@ -76,6 +76,8 @@ SIGNATURES = {
     "sglamd_fused_rms_row_quant": [_p, _i64, _p, _i64, _p, _f, _p, _i64, _i64, _p, _p, _p, _p, _p, _i, _i, _i, _p],
     "sglamd_silu_mul_row_quant": [_p, _i64, _p, _i64, _i64, _p, _p, _p, _i, _i, _p],
     "sglamd_per_token_quant_int8_asym": [_p, _i64, _i, _i64, _i64, _p, _p, _p, _p],
+    "sglamd_head_rows": [_p, _i, _i64, _i, _p, _p, _p],
+    "sglamd_gather_head_rows": [_p, _i, _i64, _i, _p, _p],
     "sglamd_fused_experts_few_tokens_workspace": [_i64, _i64, _i],
     "sglamd_fused_experts_few_tokens": [_p, _p, _i, _i64, _i64, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _i, _f, _p, _i64, _p],
     "sglamd_prepare_moe_input": [_p, _i64, _i, _i, _i64, _i64, _p, _p, _p, _p, _p, _p, _p],

@@ -502,6 +502,500 @@ Tensor int8_weight_sums(const Tensor& weight) {
 }
 
 // ---------------------------------------------------------------------------------------
+// heads between a projection and its attention (rotary.py and kv_cache.py state the contracts)
+// ---------------------------------------------------------------------------------------
+// The memory of a tensor, for calls that write into tensors they are given.
+struct Span {
+  const char* name;
+  const uint8_t *begin, *end;  // all of it lies in [begin, end)
+  int64_t item, dims = 0, sizes[4] = {}, strides[4] = {};  // bytes; dimensions of more than one element
+  Span(const char* name_, const Tensor& t) : name(name_), begin((const uint8_t*)t.data_ptr()), end(begin), item(t.element_size()) {
+    if (t.numel() == 0) return;
+    end += item;
+    for (int64_t d = 0; d < t.dim(); d++)
+      if (t.size(d) > 1) {
+        sizes[dims] = t.size(d), strides[dims] = t.stride(d) * item;
+        end += (sizes[dims] - 1) * strides[dims];
+        dims++;
+      }
+  }
+  // what the dimensions that lie closer than `step` reach over; -1 when a further one is no multiple of it
+  int64_t reach(int64_t step) const {
+    int64_t r = item;
+    for (int64_t d = 0; d < dims; d++) {
+      if (strides[d] < step) r += (sizes[d] - 1) * strides[d];
+      else if (strides[d] % step) return -1;
+    }
+    return r;
+  }
+  bool same(const Span& o) const {
+    return begin == o.begin && dims == o.dims && std::equal(sizes, sizes + dims, o.sizes) && std::equal(strides, strides + dims, o.strides);
+  }
+};
+
+// Whether two spans share no byte: apart, or side by side within every step of a stride of theirs (views of one row).
+bool disjoint(const Span& a, const Span& b) {
+  if (a.begin == a.end || b.begin == b.end || a.end <= b.begin || b.end <= a.begin) return true;
+  for (const Span* of : {&a, &b})
+    for (int64_t d = 0; d < of->dims; d++) {
+      const int64_t step = of->strides[d];
+      if (step <= 0) continue;
+      const int64_t ra = a.reach(step), rb = b.reach(step);
+      const int64_t at = ((b.begin - a.begin) % step + step) % step;
+      if (ra >= 0 && rb >= 0 && ra <= at && at + rb <= step) return true;
+    }
+  return false;
+}
+
+// Whether no element of a tensor shares its place with another one.
+bool is_apart(const Span& s) {
+  int64_t order[4] = {0, 1, 2, 3}, reach = s.item;
+  std::sort(order, order + s.dims, [&](int64_t x, int64_t y) { return s.strides[x] < s.strides[y]; });
+  for (int64_t i = 0; i < s.dims; i++) {
+    if (s.strides[order[i]] < reach) return false;
+    reach += (s.sizes[order[i]] - 1) * s.strides[order[i]];
+  }
+  return true;
+}
+
+// An address for the C interface, which wants one: memory without elements has none, and is not followed.
+void* address(const Tensor& t) {
+  static char nothing;
+  return t.numel() ? t.data_ptr() : &nothing;
+}
+
+// One call: its tensors, what it writes, and the structures of the C interface.
+struct HeadsCall {
+  const char* op;
+  sglamd_heads part[4] = {};
+  sglamd_gather back[2] = {};
+  int parts = 0;
+  sglamd_rotation rotation = {};
+  sglamd_slots slots = {};
+  const Tensor* first = nullptr;
+  std::vector<const Tensor*> reads, writes;
+  std::vector<const char*> read_names, write_names;
+  std::vector<std::pair<size_t, size_t>> in_place;  // (read, write) that may be one and the same tensor
+
+  explicit HeadsCall(const char* name) : op(name) {}
+
+  void reading(const Tensor& t, const char* name) {
+    if (!first) first = &t;
+    reads.push_back(&t), read_names.push_back(name);
+  }
+  void writing(const Tensor& t, const char* name) {
+    if (!first) first = &t;
+    writes.push_back(&t), write_names.push_back(name);
+  }
+
+  static void check_heads(const Tensor& t, const char* name, int64_t tokens, ScalarType type) {
+    TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, head size]");
+    TORCH_CHECK(t.size(0) == tokens, name, " must have as many tokens as the other tensors");
+    TORCH_CHECK(is_half(type), name, " must be Half or BFloat16");
+    TORCH_CHECK(t.scalar_type() == type, name, " must have the dtype of the other heads");
+    check_width(t, name);
+  }
+  static void check_width(const Tensor& t, const char* name) {
+    const int64_t dim = t.size(-1);
+    TORCH_CHECK(dim > 0 && dim <= 1024 && dim % 2 == 0, name, ": rows of ", dim, " values: even sizes up to 1024 are served");
+    TORCH_CHECK(t.stride(-1) == 1, name, " rows must be contiguous");
+  }
+
+  // The rotation by a table of `cos_sin.size(1)` cosines and sines.
+  void rotate_by(const Tensor& positions, const Tensor& cos_sin, bool interleaved, const optional<std::vector<int64_t>>& sections, bool alternating,
+                 int64_t tokens, ScalarType type) {
+    TORCH_CHECK(cos_sin.dim() == 2, "cos_sin must be [positions, rotated width]");
+    const int64_t width = cos_sin.size(1);
+    TORCH_CHECK(width > 0 && width % 2 == 0 && width <= 1024, "cos_sin: a rotated width of ", width, ": even, 2 to 1024");
+    TORCH_CHECK(cos_sin.stride(1) == 1, "cos_sin rows must be contiguous");
+    TORCH_CHECK(cos_sin.scalar_type() == at::kFloat || cos_sin.scalar_type() == type, "cos_sin must be Float32 or of the heads' dtype");
+    TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "positions must be Int or Long");
+    rotation.axes = 1;
+    if (sections) {
+      const int64_t axes = (int64_t)sections->size();
+      TORCH_CHECK(axes >= 1 && axes <= 4, "sections of one to four axes are served");
+      TORCH_CHECK(positions.dim() == 2 && positions.size(0) == axes && positions.size(1) == tokens, "positions must be [axes, tokens]");
+      int64_t sum = 0;
+      for (int64_t k = 0; k < axes; k++) {
+        TORCH_CHECK((*sections)[k] >= 0 && (*sections)[k] <= width, "sections must not be negative nor wider than the table");
+        sum += (*sections)[k];
+        rotation.sections[k] = (int32_t)(*sections)[k];
+      }
+      TORCH_CHECK(sum == width / 2, "sections must add up to the ", width / 2, " rotated pairs, but give ", sum);
+      if (alternating)
+        for (int64_t k = 1; k < axes; k++)
+          TORCH_CHECK((*sections)[k] == 0 || k + axes * ((*sections)[k] - 1) < width / 2, "alternating sections: axis ", k, " has no ",
+                      (*sections)[k], " turns in ", width / 2, " pairs");
+      rotation.axes = (int)axes;
+      rotation.axis_stride = positions.stride(0);
+    } else {
+      TORCH_CHECK(!alternating, "alternating axes need their sections");
+      TORCH_CHECK(positions.dim() == 1 && positions.size(0) == tokens, "positions must be [tokens], or [axes, tokens] with their sections");
+    }
+    rotation.position_stride = positions.stride(-1);
+    rotation.width = width, rotation.interleaved = interleaved, rotation.alternating = alternating;
+    rotation.table_dtype = tag(cos_sin.scalar_type()), rotation.table_rows = cos_sin.size(0), rotation.table_stride = cos_sin.stride(0);
+    rotation.positions_dtype = tag(positions.scalar_type());
+    reading(positions, "positions");
+    reading(cos_sin, "cos_sin");
+  }
+
+  // Heads that are read; `rows` of a 2D tensor are heads too, one per token.
+  sglamd_heads& add(const Tensor& x, const char* name, bool rotate) {
+    sglamd_heads& h = part[parts++];
+    const bool rows = x.dim() == 2;
+    h.x_token = x.stride(0), h.x_head = rows ? 0 : x.stride(1), h.heads = rows ? 1 : x.size(1), h.dim = x.size(-1);
+    h.rotate = rotate;
+    TORCH_CHECK(!rotate || rotation.width <= h.dim, "cos_sin: a rotated width of ", rotation.width, " for ", name, " of ", h.dim, " values");
+    reading(x, name);
+    return h;
+  }
+  void norm(sglamd_heads& h, const Tensor& w, const char* name, double eps, ScalarType type) {
+    TORCH_CHECK(w.dim() == 1 && w.numel() == h.dim && w.is_contiguous(), name, " must be contiguous [", h.dim, "]");
+    TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == type, name, " must be Float32 or of the heads' dtype");
+    TORCH_CHECK(eps >= 0 && std::isfinite((float)eps), "epsilon must be finite and not negative");
+    h.weight_dtype = tag(w.scalar_type()), h.eps = (float)eps;
+    reading(w, name);
+  }
+  // Rows in 16 bits: a tensor that is given (it may be x itself), or a new one by `allocate`.
+  void out(const sglamd_heads&, const Tensor& x, const optional<Tensor>& given, const char* name) {
+    if (!given) return;
+    TORCH_CHECK(given->sizes() == x.sizes() && given->scalar_type() == x.scalar_type(), name, " must match its input");
+    check_width(*given, name);
+    in_place.push_back({reads.size() - 1, writes.size()});
+    writing(*given, name);
+  }
+  static Tensor allocate(const Tensor& x, const optional<Tensor>& given) { return given ? *given : at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous); }
+  static void point(sglamd_heads& h, const Tensor& x, const Tensor& out) {
+    h.out = address(out), h.out_token = out.stride(0), h.out_head = x.dim() == 2 ? 0 : out.stride(1);
+  }
+
+  void take_slots(const Tensor& s, const char* name = "slots") {
+    TORCH_CHECK(s.dim() == 1, name, " must be 1D");
+    TORCH_CHECK(s.scalar_type() == at::kInt || s.scalar_type() == at::kLong, name, " must be Int or Long");
+    slots.slots_dtype = tag(s.scalar_type()), slots.slot_stride = s.stride(0), slots.page_size = -1;
+    reading(s, name);
+  }
+  // The places of a cache's rows: [slots, ...] or [pages, page size, ...], `row_dims` dimensions to a row.
+  template <typename H>
+  void take_cache(H& h, const Tensor& c, const char* name, int64_t row_dims, bool written) {
+    const bool paged = c.dim() == row_dims + 2;
+    TORCH_CHECK(paged || c.dim() == row_dims + 1, name, " must be [slots, ...] or [pages, page size, ...] of the rows");
+    const int64_t pages = c.size(0), page = paged ? c.size(1) : 1;
+    TORCH_CHECK(page > 0, name, " pages must not be empty");
+    TORCH_CHECK(slots.page_size < 0 || (slots.page_size == page && slots.pages == pages), name, " must have the pages of the other cache");
+    TORCH_CHECK(c.size(-1) == h.dim && (row_dims == 1 || c.size(-2) == h.heads), name, " rows must be [", h.heads, ", ", h.dim, "]");
+    TORCH_CHECK(c.stride(-1) == 1 || h.dim == 1, name, " rows must be contiguous");
+    TORCH_CHECK(pages < (1ll << 31) && page < (1ll << 31) && pages * page < (1ll << 31), name, ": fewer than 2^31 slots are served");
+    slots.page_size = page, slots.pages = pages;
+    h.cache_dtype = tag(c.scalar_type());
+    h.cache_page = c.stride(0), h.cache_slot = paged ? c.stride(1) : 0, h.cache_head = row_dims == 1 ? 0 : c.stride(-2);
+    if (written) writing(c, name);
+    else reading(c, name);
+  }
+  // The scale of an 8-bit cache: one number, one per head, or one per row (per 128 values of a row: `groups`) in slots of its own.
+  template <typename H>
+  void take_scale(H& h, const Tensor& c, const optional<Tensor>& scale, const char* name, bool groups, ScalarType type, bool written) {
+    if (is_half(c.scalar_type())) {
+      TORCH_CHECK(c.scalar_type() == type, name, ": a 16-bit cache must have the dtype of the heads");
+      TORCH_CHECK(!scale, name, " goes with 8-bit caches");
+      return;
+    }
+    TORCH_CHECK(c.scalar_type() == kFp8 || c.scalar_type() == at::kChar, "a cache must be Float8_e4m3fn, Char or of the heads' dtype");
+    TORCH_CHECK(scale, name, " is needed by an 8-bit cache");
+    TORCH_CHECK(scale->scalar_type() == at::kFloat, name, " must be Float32");
+    if (scale->dim() <= 1) {
+      TORCH_CHECK(c.scalar_type() == kFp8, name, ": Char rows have scales of their own");
+      TORCH_CHECK(scale->numel() == 1 || scale->numel() == h.heads, name, " must be one number, or one per head");
+      h.given_head = scale->numel() == 1 ? 0 : scale->stride(0);
+      reading(*scale, name);
+      return;
+    }
+    const int64_t places = c.dim() - (groups ? 1 : 2);  // [slots] or [pages, page size]
+    TORCH_CHECK(scale->dim() == places + 1 && std::equal(c.sizes().begin(), c.sizes().begin() + places, scale->sizes().begin()), name,
+                " must have the cache's slots");
+    h.scales_page = scale->stride(0), h.scales_slot = places == 2 ? scale->stride(1) : 0, h.scale_group = h.dim;
+    if (groups) {
+      TORCH_CHECK(scale->size(-1) == 1 || (h.dim % 128 == 0 && scale->size(-1) == h.dim / 128), name, " must be one per row, or one per 128 values");
+      h.scales_group = scale->stride(-1);
+      if (scale->size(-1) != 1) h.scale_group = 128;
+    } else {
+      TORCH_CHECK(scale->size(-1) == h.heads, name, " must be one per head of a row");
+      h.scales_head = scale->stride(-1);
+    }
+    if (written) writing(*scale, name);
+    else reading(*scale, name);
+  }
+  template <typename H>
+  static void point_scale(H& h, const optional<Tensor>& scale) {
+    if (!scale) return;
+    if (scale->dim() <= 1) h.given_scale = (float*)address(*scale);
+    else h.scales = (float*)address(*scale);
+  }
+
+  // What the shapes do not say.  There is no torch.ops schema: who has to see an operator is refused.
+  void check_tensors() const {
+    bool observed = is_observed();
+    for (const auto* list : {&reads, &writes})
+      for (const Tensor* t : *list) observed = observed || (t->is_cuda() && is_observed(*t));
+    if (observed)
+      C10_THROW_ERROR(NotImplementedError, std::string(op) + " has no gradient and takes plain tensors only, outside of tracers and "
+                                                             "transforms (call it under torch.no_grad())");
+    std::vector<Span> from, to;
+    from.reserve(reads.size()), to.reserve(writes.size());
+    for (size_t i = 0; i < writes.size(); i++) to.emplace_back(write_names[i], *writes[i]);
+    if (!to.empty())
+      for (size_t i = 0; i < reads.size(); i++) from.emplace_back(read_names[i], *reads[i]);
+    for (size_t i = 0; i < to.size(); i++) {
+      TORCH_CHECK(is_apart(to[i]), to[i].name, " must not be expanded or overlap itself");
+      for (size_t j = 0; j < i; j++) TORCH_CHECK(disjoint(to[i], to[j]), to[i].name, " must not overlap ", to[j].name);
+      for (size_t j = 0; j < from.size(); j++) {
+        const bool may = std::find(in_place.begin(), in_place.end(), std::make_pair(j, i)) != in_place.end() && to[i].same(from[j]);
+        TORCH_CHECK(may || disjoint(to[i], from[j]), to[i].name, " must not overlap ", from[j].name);
+      }
+    }
+    for (const auto* list : {&reads, &writes})
+      for (const Tensor* t : *list) {
+        TORCH_CHECK(t->is_cuda(), op, ": every tensor must be a CUDA tensor");
+        TORCH_CHECK(t->device() == first->device(), op, ": every tensor must be on the same device");
+      }
+  }
+  void launch(int64_t tokens, ScalarType type, bool rotated) {
+    if (tokens)
+      check(sglamd_head_rows(part, parts, tokens, tag(type), rotated ? &rotation : nullptr, slots.slots ? &slots : nullptr, stream_of(*first)));
+    for (const Tensor* t : writes) written_in_place(*t);
+  }
+};
+
+std::tuple<Tensor, optional<Tensor>> rotate_heads(const char* op, const Tensor& q, const optional<Tensor>& k, const optional<Tensor>& q_weight,
+                                                  const optional<Tensor>& k_weight, double eps, const Tensor& positions, const Tensor& cos_sin,
+                                                  bool interleaved, const optional<std::vector<int64_t>>& sections, bool alternating,
+                                                  const optional<Tensor>& q_out, const optional<Tensor>& k_out) {
+  HeadsCall call(op);
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head size]");
+  const int64_t tokens = q.size(0);
+  const ScalarType type = q.scalar_type();
+  HeadsCall::check_heads(q, "q", tokens, type);
+  call.rotate_by(positions, cos_sin, interleaved, sections, alternating, tokens, type);
+  sglamd_heads& hq = call.add(q, "q", true);
+  call.out(hq, q, q_out, "q_out");
+  if (q_weight) call.norm(hq, *q_weight, "q_weight", eps, type);
+  TORCH_CHECK(k || !k_out, "k_out goes with k");
+  if (k) {
+    HeadsCall::check_heads(*k, "k", tokens, type);
+    sglamd_heads& hk = call.add(*k, "k", true);
+    call.out(hk, *k, k_out, "k_out");
+    if (k_weight) call.norm(hk, *k_weight, "k_weight", eps, type);
+  }
+  call.check_tensors();
+  const c10::DeviceGuard guard(q.device());
+  call.rotation.cos_sin = address(cos_sin), call.rotation.positions = address(positions);
+  const Tensor q_to = HeadsCall::allocate(q, q_out);
+  optional<Tensor> k_to;
+  hq.x = q.data_ptr(), hq.weight = q_weight ? q_weight->data_ptr() : nullptr;
+  HeadsCall::point(hq, q, q_to);
+  if (k) {
+    k_to = HeadsCall::allocate(*k, k_out);
+    sglamd_heads& hk = call.part[1];
+    hk.x = k->data_ptr(), hk.weight = k_weight ? k_weight->data_ptr() : nullptr;
+    HeadsCall::point(hk, *k, *k_to);
+  }
+  call.launch(tokens, type, true);
+  return {q_to, k_to};
+}
+
+std::tuple<Tensor, optional<Tensor>> rotate_qk(const Tensor& q, const optional<Tensor>& k, const Tensor& positions, const Tensor& cos_sin,
+                                               bool interleaved, const optional<std::vector<int64_t>>& sections, bool alternating,
+                                               const optional<Tensor>& q_out, const optional<Tensor>& k_out) {
+  return rotate_heads("rotate_qk", q, k, {}, {}, 0.0, positions, cos_sin, interleaved, sections, alternating, q_out, k_out);
+}
+
+std::tuple<Tensor, optional<Tensor>> norm_rotate_qk(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight, double eps,
+                                                    const Tensor& positions, const Tensor& cos_sin, bool interleaved,
+                                                    const optional<std::vector<int64_t>>& sections, bool alternating, const optional<Tensor>& q_out,
+                                                    const optional<Tensor>& k_out) {
+  return rotate_heads("norm_rotate_qk", q, k, q_weight, k_weight, eps, positions, cos_sin, interleaved, sections, alternating, q_out, k_out);
+}
+
+std::tuple<optional<Tensor>, optional<Tensor>> append_kv(
+    const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots, const optional<Tensor>& k_scale,
+    const optional<Tensor>& v_scale, const optional<Tensor>& q, const optional<Tensor>& positions, const optional<Tensor>& cos_sin, bool interleaved,
+    const optional<std::vector<int64_t>>& sections, bool alternating, const optional<Tensor>& q_weight, const optional<Tensor>& k_weight, double eps,
+    const optional<Tensor>& q_out, const optional<Tensor>& k_out) {
+  HeadsCall call("append_kv");
+  TORCH_CHECK(k.dim() == 3, "k must be [tokens, heads, head size]");
+  const int64_t tokens = k.size(0);
+  const ScalarType type = k.scalar_type();
+  HeadsCall::check_heads(k, "k", tokens, type);
+  HeadsCall::check_heads(v, "v", tokens, type);
+  TORCH_CHECK(positions.has_value() == cos_sin.has_value(), "positions and cos_sin go together");
+  TORCH_CHECK(positions || (!sections && !alternating && !interleaved), "a rotation needs positions and cos_sin");
+  const bool rotated = positions.has_value();
+  TORCH_CHECK(!q || rotated || q_weight, "q is only taken to be rotated or normalised");
+  TORCH_CHECK(q || (!q_out && !q_weight), "q_out and q_weight go with q");
+  if (rotated) call.rotate_by(*positions, *cos_sin, interleaved, sections, alternating, tokens, type);
+  call.take_slots(slots);
+  TORCH_CHECK(slots.size(0) == tokens, "slots must be one per token");
+  sglamd_heads& hk = call.add(k, "k", rotated);
+  call.out(hk, k, k_out, "k_out");
+  if (k_weight) call.norm(hk, *k_weight, "k_weight", eps, type);
+  call.take_cache(hk, k_cache, "k_cache", 2, true);
+  call.take_scale(hk, k_cache, k_scale, "k_scale", false, type, true);
+  sglamd_heads& hv = call.add(v, "v", false);
+  call.take_cache(hv, v_cache, "v_cache", 2, true);
+  call.take_scale(hv, v_cache, v_scale, "v_scale", false, type, true);
+  if (q) {
+    HeadsCall::check_heads(*q, "q", tokens, type);
+    sglamd_heads& hq = call.add(*q, "q", rotated);
+    call.out(hq, *q, q_out, "q_out");
+    if (q_weight) call.norm(hq, *q_weight, "q_weight", eps, type);
+  }
+  call.check_tensors();
+  const c10::DeviceGuard guard(k.device());
+  if (rotated) call.rotation.cos_sin = address(*cos_sin), call.rotation.positions = address(*positions);
+  call.slots.slots = address(slots);
+  hk.x = k.data_ptr(), hk.weight = k_weight ? k_weight->data_ptr() : nullptr, hk.cache = address(k_cache);
+  HeadsCall::point_scale(hk, k_scale);
+  if (k_out) HeadsCall::point(hk, k, *k_out);
+  hv.x = v.data_ptr(), hv.cache = address(v_cache);
+  HeadsCall::point_scale(hv, v_scale);
+  optional<Tensor> q_to;
+  if (q) {
+    q_to = HeadsCall::allocate(*q, q_out);
+    sglamd_heads& hq = call.part[2];
+    hq.x = q->data_ptr(), hq.weight = q_weight ? q_weight->data_ptr() : nullptr;
+    HeadsCall::point(hq, *q, *q_to);
+  }
+  call.launch(tokens, type, rotated);
+  return {q_to, k_out};
+}
+
+optional<Tensor> append_latent(const Tensor& latent, const Tensor& rope, const Tensor& latent_cache, const Tensor& rope_cache, const Tensor& slots,
+                               const Tensor& positions, const Tensor& cos_sin, const optional<Tensor>& weight, double eps, bool interleaved,
+                               const optional<Tensor>& scale, const optional<Tensor>& rope_scale, const optional<Tensor>& q_rope,
+                               const optional<Tensor>& q_out) {
+  HeadsCall call("append_latent");
+  TORCH_CHECK(latent.dim() == 2 && rope.dim() == 2 && rope.size(0) == latent.size(0), "latent and rope must be [tokens, values]");
+  const int64_t tokens = latent.size(0);
+  const ScalarType type = latent.scalar_type();
+  TORCH_CHECK(is_half(type) && rope.scalar_type() == type, "latent and rope must be Half or BFloat16, both the same");
+  HeadsCall::check_width(latent, "latent");
+  HeadsCall::check_width(rope, "rope");
+  TORCH_CHECK(q_rope || !q_out, "q_out goes with q_rope");
+  call.rotate_by(positions, cos_sin, interleaved, {}, false, tokens, type);
+  call.take_slots(slots);
+  TORCH_CHECK(slots.size(0) == tokens, "slots must be one per token");
+  sglamd_heads& hl = call.add(latent, "latent", false);
+  if (weight) call.norm(hl, *weight, "weight", eps, type);
+  call.take_cache(hl, latent_cache, "latent_cache", 1, true);
+  call.take_scale(hl, latent_cache, scale, "scale", true, type, true);
+  sglamd_heads& hr = call.add(rope, "rope", true);
+  call.take_cache(hr, rope_cache, "rope_cache", 1, true);
+  TORCH_CHECK(rope_cache.scalar_type() != at::kChar && (!rope_scale || rope_scale->dim() <= 1),
+              "rope_cache: the rotated part is kept in 16 bits or in Float8_e4m3fn with a given scale");
+  call.take_scale(hr, rope_cache, rope_scale, "rope_scale", true, type, true);
+  if (q_rope) {
+    HeadsCall::check_heads(*q_rope, "q_rope", tokens, type);
+    sglamd_heads& hq = call.add(*q_rope, "q_rope", true);
+    call.out(hq, *q_rope, q_out, "q_out");
+  }
+  call.check_tensors();
+  const c10::DeviceGuard guard(latent.device());
+  call.rotation.cos_sin = address(cos_sin), call.rotation.positions = address(positions);
+  call.slots.slots = address(slots);
+  hl.x = latent.data_ptr(), hl.weight = weight ? weight->data_ptr() : nullptr, hl.cache = address(latent_cache);
+  HeadsCall::point_scale(hl, scale);
+  hr.x = rope.data_ptr(), hr.cache = address(rope_cache);
+  HeadsCall::point_scale(hr, rope_scale);
+  optional<Tensor> q_to;
+  if (q_rope) {
+    q_to = HeadsCall::allocate(*q_rope, q_out);
+    call.part[2].x = q_rope->data_ptr();
+    HeadsCall::point(call.part[2], *q_rope, *q_to);
+  }
+  call.launch(tokens, type, true);
+  return q_to;
+}
+
+// Rows of one or two caches; `out` [rows, heads, dim] each.
+void gather_into(HeadsCall& call, int64_t rows, ScalarType type, const Tensor& first_cache, const Tensor& second_cache,
+                 const optional<Tensor>& first_scale, const optional<Tensor>& second_scale, const Tensor& first_out, const Tensor& second_out,
+                 const Tensor& slots) {
+  call.slots.slots = address(slots);
+  const Tensor* caches[2] = {&first_cache, &second_cache};
+  const optional<Tensor>* scales[2] = {&first_scale, &second_scale};
+  const Tensor* outs[2] = {&first_out, &second_out};
+  for (int i = 0; i < 2; i++) {
+    sglamd_gather& g = call.back[i];
+    g.cache = address(*caches[i]);
+    HeadsCall::point_scale(g, *scales[i]);
+    g.out = address(*outs[i]), g.out_row = outs[i]->stride(0), g.out_head = outs[i]->dim() == 2 ? 0 : outs[i]->stride(1);
+  }
+  if (rows) check(sglamd_gather_head_rows(call.back, 2, rows, tag(type), &call.slots, stream_of(slots)));
+  for (const Tensor* t : call.writes) written_in_place(*t);
+}
+
+void check_gather(const Tensor& cache, const char* name, int64_t row_dims, sglamd_gather& g) {
+  TORCH_CHECK(cache.dim() == row_dims + 1 || cache.dim() == row_dims + 2, name, " must be [slots, ...] or [pages, page size, ...] of the rows");
+  g.heads = row_dims == 1 ? 1 : cache.size(-2), g.dim = cache.size(-1);
+  TORCH_CHECK(g.dim > 0 && g.dim <= 1024, name, ": rows of ", g.dim, " values: up to 1024 are served");
+}
+
+std::tuple<Tensor, Tensor> gather_kv(const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots, ScalarType type, const optional<Tensor>& k_scale,
+                                     const optional<Tensor>& v_scale, const optional<Tensor>& k_out, const optional<Tensor>& v_out) {
+  HeadsCall call("gather_kv");
+  TORCH_CHECK(is_half(type), "dtype must be Half or BFloat16");
+  call.take_slots(slots);
+  const int64_t rows = slots.size(0);
+  const auto take = [&](int i, const Tensor& cache, const char* name, const optional<Tensor>& scale, const char* scale_name,
+                        const optional<Tensor>& out, const char* out_name) {
+    sglamd_gather& g = call.back[i];
+    check_gather(cache, name, 2, g);
+    call.take_cache(g, cache, name, 2, false);
+    call.take_scale(g, cache, scale, scale_name, false, type, false);
+    if (!out) return;
+    TORCH_CHECK(out->dim() == 3 && out->size(0) == rows && out->size(1) == g.heads && out->size(2) == g.dim && out->scalar_type() == type, out_name,
+                " must be [rows, heads, head size] of dtype");
+    TORCH_CHECK(out->stride(2) == 1 || g.dim == 1, out_name, " rows must be contiguous");
+    call.writing(*out, out_name);
+  };
+  take(0, k_cache, "k_cache", k_scale, "k_scale", k_out, "k_out");
+  take(1, v_cache, "v_cache", v_scale, "v_scale", v_out, "v_out");
+  call.check_tensors();
+  const c10::DeviceGuard guard(k_cache.device());
+  const Tensor k_to = k_out ? *k_out : empty({rows, call.back[0].heads, call.back[0].dim}, type, k_cache);
+  const Tensor v_to = v_out ? *v_out : empty({rows, call.back[1].heads, call.back[1].dim}, type, v_cache);
+  gather_into(call, rows, type, k_cache, v_cache, k_scale, v_scale, k_to, v_to, slots);
+  return {k_to, v_to};
+}
+
+Tensor gather_latent(const Tensor& latent_cache, const Tensor& rope_cache, const Tensor& slots, ScalarType type, const optional<Tensor>& scale,
+                     const optional<Tensor>& rope_scale, const optional<Tensor>& out) {
+  HeadsCall call("gather_latent");
+  TORCH_CHECK(is_half(type), "dtype must be Half or BFloat16");
+  call.take_slots(slots);
+  const int64_t rows = slots.size(0);
+  check_gather(latent_cache, "latent_cache", 1, call.back[0]);
+  call.take_cache(call.back[0], latent_cache, "latent_cache", 1, false);
+  call.take_scale(call.back[0], latent_cache, scale, "scale", true, type, false);
+  check_gather(rope_cache, "rope_cache", 1, call.back[1]);
+  call.take_cache(call.back[1], rope_cache, "rope_cache", 1, false);
+  call.take_scale(call.back[1], rope_cache, rope_scale, "rope_scale", true, type, false);
+  const int64_t split = call.back[0].dim, width = split + call.back[1].dim;
+  if (out) {
+    TORCH_CHECK(out->dim() == 2 && out->size(0) == rows && out->size(1) == width && out->scalar_type() == type, "out must be [rows, ", width,
+                "] of dtype");
+    TORCH_CHECK(out->stride(1) == 1, "out rows must be contiguous");
+    call.writing(*out, "out");
+  }
+  call.check_tensors();
+  const c10::DeviceGuard guard(latent_cache.device());
+  const Tensor to = out ? *out : empty({rows, width}, type, latent_cache);
+  gather_into(call, rows, type, latent_cache, rope_cache, scale, rope_scale, to.narrow(1, 0, split), to.narrow(1, split, width - split), slots);
+  return to;
+}
+
+// ---------------------------------------------------------------------------------------
 // dense GEMMs
 // ---------------------------------------------------------------------------------------
 // fp32 split-K scratch when the library can use one for this shape; from the caching allocator, so calls on other
@@ -1462,6 +1956,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("silu_mul_row_quant", &silu_mul_row_quant, Unlocked());
   m.def("per_token_quant_int8_asym", &per_token_quant_int8_asym, Unlocked());
   m.def("int8_weight_sums", &int8_weight_sums, Unlocked());
+  m.def("rotate_qk", &rotate_qk, Unlocked());
+  m.def("norm_rotate_qk", &norm_rotate_qk, Unlocked());
+  m.def("append_kv", &append_kv, Unlocked());
+  m.def("append_latent", &append_latent, Unlocked());
+  m.def("gather_kv", &gather_kv, Unlocked());
+  m.def("gather_latent", &gather_latent, Unlocked());
   m.def("int8_scaled_mm_azp", &int8_scaled_mm_azp, Unlocked());
   m.def("int8_linear", &int8_linear, Unlocked());
   m.def("experts_few_tokens", &experts_few_tokens, Unlocked());
