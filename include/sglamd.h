@@ -679,7 +679,7 @@ typedef struct {
   int64_t scales_page, scales_slot, scales_head, scales_group, scale_group;
 } sglamd_heads;
 
-/* One to four tensors of heads of the same tokens and of one type (dtype F16 or BF16).  `parts`, `rotation` (NULL: nothing is
+/* One to three tensors of heads of the same tokens and of one type (dtype F16 or BF16).  `parts`, `rotation` (NULL: nothing is
  * rotated) and `slots` (NULL: no cache) are host structures, read before the call returns. */
 int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_t tokens, int dtype, const sglamd_rotation* rotation,
                      const sglamd_slots* slots, void* stream);

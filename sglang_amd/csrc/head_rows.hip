@@ -7,8 +7,15 @@
 //
 // Everything between the load of a head and its stores is in fp32 and rounded once, to the type of the row that is written.
 //
-// All of it is bound by HBM at prompt sizes (a few operations per value, each value read once and written once) and by the
-// launch at decode sizes, so the aim is one launch for everything that a layer does between its projection and its attention.
+// All of it is bound by HBM at prompt sizes (some ten operations per value, each value read once and written once) and by the launch
+// at decode sizes, so one launch does everything that a layer needs between its projection and its attention.  Measured
+// against a copy of as many bytes (5.05 TB/s): 8191 tokens of 64 + 2 x 8 heads of 128, rotated, into e4m3 rows 5.2 TB/s; 4096 tokens
+// of 128 rotary parts, 128 bytes in each 384, 4.4 (a copy of such pieces 4.5); gathered int8 rows 5.0; heads with a norm 4.3 to 4.5.
+// What decided it, in this order: pieces in words (a piece of eight 16-bit values that may not be there was held in
+// eight registers), one head per lane group in at most 64 registers instead of four in 160 (4.3 to 5.2 TB/s), loads without
+// conditions (a condition between two loads makes the first wait for both), and the kernel's arguments touched at the start.
+#include <utility>
+
 #include "row_out.h"
 
 namespace sglamd {
@@ -24,27 +31,26 @@ struct HeadPart {
   uint8_t* cache;  // rows of the slots, or null; strides in bytes
   int64_t cache_page, cache_slot, cache_head;
   const float* given;  // scale, one or one per head
-  float* scales;       // scales that are found here, one per `scale_units` units of a row
+  float* scales;       // scales that are found here, one per row or per 128 values of it
   int64_t given_head, scales_page, scales_slot, scales_head, scales_group;
   float eps, inv_dim;
-  uint32_t first_block, groups;  // lane groups of this part: tokens * per_token
+  uint32_t groups;  // lane groups of this part: tokens * per_token
   FastDiv per_token_div;
   int per_token, heads, units, rot_units;
-  int lanes_log2, scale_lanes_log2, scale_units;
-  int kind, w_is_f32;
+  int lanes_log2, kind, w_is_f32, grouped;  // grouped: a scale per 128 values
 };
 
-constexpr int MAX_PARTS = 4;
+constexpr int MAX_PARTS = 3;
 
 struct HeadArgs {
   HeadPart part[MAX_PARTS];
-  int parts;
+  uint32_t first_block[MAX_PARTS];  // of each part; behind the last block for parts that are not there
   // rotation
   const void* table;
   int64_t table_stride, table_rows, axis_stride, position_stride;
   const void* positions;
-  int pairs, table_is_f32, positions_are_i64, axes, alternating;
-  int section[4], axis_inv;  // blocks: where axes 1, 2 and 3 begin; alternating: pairs of each axis, 65536 / axes rounded up
+  int pairs, table_is_f32, positions_are_i64, axes;
+  uint32_t axis_bits[2][16];  // the axis of each pair, its low and its high bit
   // slots
   const void* slots;
   int64_t slot_stride, num_slots;
@@ -52,20 +58,50 @@ struct HeadArgs {
   FastDiv page_div;
 };
 
+// Every line of the kernel's arguments into the scalar cache, in one round trip: they lie in memory that the caches below do not
+// hold, and line after line, each where its fields are first used, a workgroup waits about a microsecond for each.
+__device__ __forceinline__ int touched(uint32_t word) {
+  asm volatile("" ::"s"(word));
+  return 0;
+}
+template <typename ARGS, int... I>
+__device__ __forceinline__ void touch_lines(const ARGS& a, std::integer_sequence<int, I...>) {
+  const uint32_t w[] = {((const uint32_t*)&a)[16 * I]...};
+  const int done[] = {touched(w[I])...};
+  (void)done;
+}
+template <typename ARGS>
+__device__ __forceinline__ void touch_arguments(const ARGS& a) {
+  touch_lines(a, std::make_integer_sequence<int, (sizeof(ARGS) + 63) / 64>());
+}
+
+// V 16-bit values as loaded: words, so that a piece that may not be there is held in words too.
 template <int V>
 struct Piece {
-  u16 v[V];
+  typedef uint32_t type __attribute__((ext_vector_type(V / 2)));
 };
-template <int V, typename E>
-__device__ __forceinline__ Piece<V> load_values(const E* p) {  // (global memory takes any alignment)
-  Piece<V> v;
-  __builtin_memcpy(&v, p, sizeof(v));
-  return v;
+template <>
+struct Piece<1> {
+  typedef uint32_t type;
+};
+template <int V>
+__device__ __forceinline__ typename Piece<V>::type load_values(const u16* p) {  // (global memory takes any alignment)
+  if constexpr (V == 1) {
+    return *p;
+  } else {
+    typename Piece<V>::type v;
+    __builtin_memcpy(&v, p, sizeof(v));
+    return v;
+  }
 }
 template <typename T, int V>
-__device__ __forceinline__ void to_floats(const Piece<V>& p, float* f) {
+__device__ __forceinline__ void to_floats(const typename Piece<V>::type& p, float* f) {
+  if constexpr (V == 1) {
+    f[0] = T::to_f32((u16)p);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; i++) f[i] = T::to_f32(p.v[i]);
+    for (int i = 0; i < V / 2; i++) f[2 * i] = T::to_f32((u16)p[i]), f[2 * i + 1] = T::to_f32((u16)(p[i] >> 16));
+  }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_values(u16* p, const float* f) {
@@ -90,14 +126,39 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float* f, const Ro
     __builtin_memcpy(p, w, V);
   }
 }
-// V values of fp32 or of the 16-bit type, as fp32.
-template <typename T, int V>
-__device__ __forceinline__ void load_mixed(const void* base, int64_t at, bool f32, float* f) {
-  if (f32) __builtin_memcpy(f, (const float*)base + at, 4 * V);
-  else to_floats<T>(load_values<V>((const u16*)base + at), f);
+// N cosines or sines at a byte offset into the table: 32 bits, beside its address in scalar registers.
+template <typename T, int N>
+__device__ __forceinline__ void load_table(const HeadArgs& a, uint32_t at, float* f) {
+  const char* p = (const char*)a.table + at;
+  if (a.table_is_f32) __builtin_memcpy(f, p, 4 * N);
+  else to_floats<T, N>(load_values<N>((const u16*)p), f);
 }
-__device__ __forceinline__ int64_t load_index(const void* base, int64_t at, int is_i64) {
-  return is_i64 ? ((const int64_t*)base)[at] : (int64_t)((const int32_t*)base)[at];
+// Weights as fp32, ones where there are none; those of 16 bits have been loaded already.
+template <typename T, int V>
+__device__ __forceinline__ void weights(const HeadPart& p, int at, const typename Piece<V>::type& raw, float* w) {
+  if (p.w_is_f32) {
+    __builtin_memcpy(w, (const char*)p.w + (uint32_t)(4 * at), 4 * V);
+  } else {
+    to_floats<T, V>(raw, w);
+#pragma unroll
+    for (int i = 0; i < V; i++) w[i] = p.w ? w[i] : 1.f;
+  }
+}
+// An index in two words, without a branch on its type: what is loaded behind it can be waited for by itself.
+struct Index {
+  int lo, hi;
+  __device__ __forceinline__ int64_t value(int is_i64) const { return (int64_t)(uint32_t)lo | (int64_t)(is_i64 ? hi : lo >> 31) << 32; }
+};
+__device__ __forceinline__ Index load_index(const void* base, int64_t at, int is_i64) {
+  const int* p = (const int*)base + (is_i64 ? 2 * at : at);
+  return {p[0], p[is_i64 ? 1 : 0]};
+}
+
+// The values are computed here and not later, and what is loaded below is not loaded above.
+template <int V>
+__device__ __forceinline__ void pin(float* f) {
+#pragma unroll
+  for (int i = 0; i < V; i++) asm volatile("" : "+v"(f[i])::"memory");
 }
 
 // Sum and maximum over aligned groups of 2^log lanes, in all of them; `log` is the same in the whole wave.
@@ -120,59 +181,77 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v, int log) {
   return v;
 }
 
-__device__ __forceinline__ int axis_of_pair(const HeadArgs& a, int i) {
-  if (a.alternating) {
-    const int m = i - ((i * a.axis_inv) >> 16) * a.axes;  // i mod axes
-    const int n = m == 0 ? a.section[0] : m == 1 ? a.section[1] : m == 2 ? a.section[2] : a.section[3];
-    return i < a.axes * n ? m : 0;
+// Which axes the N pairs from `first` on turn by: the low and the high bits of their numbers.
+struct AxisBits {
+  uint32_t lo, hi;
+};
+template <int N>
+__device__ __forceinline__ AxisBits axes_of_pairs(const HeadArgs& a, int first) {
+  constexpr uint32_t ALL = (1u << N) - 1;
+  AxisBits b = {0, 0};
+  // (word by word, in scalar registers: vector loads of kernel arguments cross to the host's memory)
+  for (int w = 0; w * 32 < a.pairs; w++) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(a.axis_bits[0][w]), hi = __builtin_amdgcn_readfirstlane(a.axis_bits[1][w]);
+    b.lo = first >> 5 == w ? lo : b.lo;
+    b.hi = first >> 5 == w ? hi : b.hi;
   }
-  return (i >= a.section[1]) + (i >= a.section[2]) + (i >= a.section[3]);
+  return {b.lo >> (first & 31) & ALL, b.hi >> (first & 31) & ALL};
+}
+// (values and not an array: the choice of an address would put it into memory)
+template <typename E>
+__device__ __forceinline__ E of_axis(const AxisBits& b, int i, E v0, E v1, E v2, E v3) {
+  const E low = b.lo >> i & 1 ? v1 : v0, high = b.lo >> i & 1 ? v3 : v2;
+  return b.hi >> i & 1 ? high : low;
 }
 
-// Cosines and sines of pairs [first, first + V) of a token.  A position outside of the table gives NaN: nothing is read there.
-template <typename T, int V>
-__device__ __forceinline__ void load_turn(const HeadArgs& a, const int64_t (&pos)[4], int first, float* c, float* s) {
-  int ax = 0;
-  bool mixed = false;
-  if (a.axes > 1) {
-    ax = axis_of_pair(a, first);
-    if (V > 1) {
-      const bool same = pos[0] == pos[1] && (a.axes < 3 || pos[0] == pos[2]) && (a.axes < 4 || pos[0] == pos[3]);
-      mixed = !same && (a.alternating || axis_of_pair(a, first + V - 1) != ax);
+// Cosines and sines of the N pairs from `first` on, `rows` (byte offsets into the table) and `inside` for each axis.  A position
+// outside of the table gives NaN, and reads the table's first row.
+template <typename T, int N, bool AXES>
+__device__ __forceinline__ void load_turn(const HeadArgs& a, const uint32_t (&rows)[AXES ? 4 : 1], const bool (&inside)[AXES ? 4 : 1],
+                                          const AxisBits& axes, int first, float* c, float* s) {
+  const int item = a.table_is_f32 ? 4 : 2;
+  const uint32_t pair = (uint32_t)(first * item), sines = (uint32_t)(a.pairs * item);
+  if constexpr (!AXES) {
+    load_table<T, N>(a, rows[0] + pair, c);
+    load_table<T, N>(a, rows[0] + pair + sines, s);
+    if (__any(!inside[0])) {
+#pragma unroll
+      for (int i = 0; i < N; i++) c[i] = inside[0] ? c[i] : NAN, s[i] = inside[0] ? s[i] : NAN;
     }
-  }
-  const int64_t p = ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : pos[3];
-  if (!mixed) {
-    if ((uint64_t)p < (uint64_t)a.table_rows) {
-      load_mixed<T, V>(a.table, p * a.table_stride + first, a.table_is_f32, c);
-      load_mixed<T, V>(a.table, p * a.table_stride + first + a.pairs, a.table_is_f32, s);
+  } else {
+    constexpr uint32_t ALL = (1u << N) - 1;
+    // (a text token has the same position on every axis; axes in blocks change once in a while)
+    const bool same = rows[0] == rows[1] && rows[0] == rows[2] && rows[0] == rows[3];
+    if (same || ((axes.lo == 0 || axes.lo == ALL) && (axes.hi == 0 || axes.hi == ALL))) {
+      const uint32_t at = of_axis(axes, 0, rows[0], rows[1], rows[2], rows[3]) + pair;
+      load_table<T, N>(a, at, c);
+      load_table<T, N>(a, at + sines, s);
+    } else if (a.table_is_f32) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const uint32_t at = of_axis(axes, i, rows[0], rows[1], rows[2], rows[3]) + pair + 4 * i;
+        c[i] = *(const float*)((const char*)a.table + at);
+        s[i] = *(const float*)((const char*)a.table + (uint32_t)(at + sines));
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; i++) c[i] = s[i] = NAN;
+      for (int i = 0; i < N; i++) {
+        const uint32_t at = of_axis(axes, i, rows[0], rows[1], rows[2], rows[3]) + pair + 2 * i;
+        c[i] = T::to_f32(*(const u16*)((const char*)a.table + at));
+        s[i] = T::to_f32(*(const u16*)((const char*)a.table + (uint32_t)(at + sines)));
+      }
     }
-    return;
-  }
-  if constexpr (V > 1) {  // one row after the other, each pair keeps its own axis's values
+    if (__any(!(inside[0] && inside[1] && inside[2] && inside[3]))) {
 #pragma unroll
-    for (int i = 0; i < V; i++) c[i] = s[i] = NAN;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      if (k < a.axes && (uint64_t)pos[k] < (uint64_t)a.table_rows) {
-        float ck[V], sk[V];
-        load_mixed<T, V>(a.table, pos[k] * a.table_stride + first, a.table_is_f32, ck);
-        load_mixed<T, V>(a.table, pos[k] * a.table_stride + first + a.pairs, a.table_is_f32, sk);
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-          const bool mine = axis_of_pair(a, first + i) == k;
-          c[i] = mine ? ck[i] : c[i];
-          s[i] = mine ? sk[i] : s[i];
-        }
+      for (int i = 0; i < N; i++) {
+        const bool ok = of_axis(axes, i, inside[0], inside[1], inside[2], inside[3]);
+        c[i] = ok ? c[i] : NAN, s[i] = ok ? s[i] : NAN;
       }
     }
   }
 }
 
-// (f0, f1) are pieces V pairs apart, or 2 V consecutive values.
+// f0 and f1: the V values of a unit's two pieces.
 template <int V, bool ADJACENT>
 __device__ __forceinline__ void turn(float* f0, float* f1, const float* c, const float* s) {
   if constexpr (!ADJACENT || V == 1) {
@@ -208,106 +287,159 @@ __device__ __forceinline__ RowScale found_scale(uint32_t hi_bits) {
   return o;
 }
 
-// A head belongs to 2^lanes_log2 lanes, each with K units of 2 V values: V pairs of the rotated part (both halves of them, so
-// that a rotation needs no other lane), or 2 V consecutive values.  A lane group takes up to HEADS heads of one token, loads them
-// all before it waits for the first and uses the table's row and the weights for all of them.
-template <typename T, int V, int K, int HEADS, bool ADJACENT>
-__global__ __launch_bounds__(256) void head_rows_kernel(const HeadArgs a) {
-  int index = 0;
-  while (index + 1 < a.parts && blockIdx.x >= a.part[index + 1].first_block) index++;
+// A head belongs to 2^lanes_log2 lanes, each with K units of two pieces of V values.  The pieces of a unit lie half a stretch apart, a
+// stretch being the rotated part, the part behind it, or 128 values with a scale of their own: so both values of a pair are in
+// one lane, half to half or side by side, and neighbouring lanes load and store neighbouring pieces.  A lane group takes up to
+// HEADS heads of one token, loads them all before it waits for the first and uses the table's row and the weights for all of them.
+template <typename T, int V, int K, int HEADS, bool ADJACENT, bool AXES, bool NORM>
+__global__ __launch_bounds__(256, V == 8 && HEADS == 1 ? 8 : 1) void head_rows_kernel(const HeadArgs a) {
+  constexpr bool PAIRS_IN_PIECES = ADJACENT && V > 1;
+  constexpr int GROUP_UNITS = 64 / V, GROUP_LOG2 = V == 8 ? 3 : V == 4 ? 4 : 6;
+  touch_arguments(a);
+  const uint32_t block = blockIdx.x;
+  const int index = (block >= a.first_block[1]) + (block >= a.first_block[2]);
   const HeadPart& p = a.part[index];
-  const uint32_t group = ((blockIdx.x - p.first_block) << (8 - p.lanes_log2)) + (threadIdx.x >> p.lanes_log2);
+  const int lanes_log2 = p.lanes_log2;
+  const uint32_t group = ((block - a.first_block[index]) << (8 - lanes_log2)) + (threadIdx.x >> lanes_log2);
   if (group >= p.groups) return;
+  const int per_token = p.per_token, units = p.units, rot_units = p.rot_units, kind = p.kind, heads = p.heads;
   const uint32_t token = p.per_token_div.divide(group);
-  const int first_head = (int)(group - token * (uint32_t)p.per_token), lane = threadIdx.x & ((1 << p.lanes_log2) - 1);
-
-  int64_t pos[4] = {0, 0, 0, 0}, slot = -1;
-  if (p.rot_units) {
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (k < a.axes) pos[k] = load_index(a.positions, k * a.axis_stride + (int64_t)token * a.position_stride, a.positions_are_i64);
-  }
-  if (p.kind != HEADS_TO_NONE) slot = load_index(a.slots, (int64_t)token * a.slot_stride, a.slots_are_i64);
+  const int first_head = (int)(group - token * (uint32_t)per_token), lane = threadIdx.x & ((1 << lanes_log2) - 1);
 
   // where a lane's pieces lie in a head
   int at0[K], at1[K];
   bool rotated[K], real[K];
 #pragma unroll
   for (int j = 0; j < K; j++) {
-    const int u = lane + (j << p.lanes_log2);
-    real[j] = u < p.units;
-    rotated[j] = u < p.rot_units;
-    const bool halves = !ADJACENT && rotated[j];
-    at0[j] = halves ? u * V : 2 * u * V;
-    at1[j] = at0[j] + (halves ? a.pairs : V);
+    const int wanted = lane + (j << lanes_log2), u = min(wanted, units - 1);
+    real[j] = wanted < units;
+    rotated[j] = u < rot_units;
+    if (ADJACENT && V == 1 && rotated[j]) {
+      at0[j] = 2 * u;
+      at1[j] = at0[j] + 1;
+    } else if (p.grouped) {
+      at0[j] = ((u >> GROUP_LOG2) << 7) + (u & (GROUP_UNITS - 1)) * V;
+      at1[j] = at0[j] + 64;
+    } else {
+      at0[j] = (rotated[j] ? u : u + rot_units) * V;
+      at1[j] = at0[j] + (rotated[j] ? rot_units : units - rot_units) * V;
+    }
   }
 
-  Piece<V> raw0[HEADS][K], raw1[HEADS][K];
-  const u16* x = p.x + (int64_t)token * p.x_token;
+  // Positions first: the table's rows hang on them.  Then the heads, all at once and without a condition (lanes and heads that are
+  // none read the last one), so that neither waits for the other.
+  AxisBits axes0[K] = {}, axes1[K] = {};
+  Index pos[AXES ? 4 : 1] = {}, slot_index = {};
+  if (rot_units) {
 #pragma unroll
-  for (int h = 0; h < HEADS; h++) {
-    const int head = first_head + h * p.per_token;
+    for (int k = 0; k < (AXES ? 4 : 1); k++)
+      pos[k] = load_index(a.positions, (AXES ? min(k, a.axes - 1) * a.axis_stride : 0) + (int64_t)token * a.position_stride, a.positions_are_i64);
+    if constexpr (AXES) {
 #pragma unroll
-    for (int j = 0; j < K; j++) {
-      raw0[h][j] = {}, raw1[h][j] = {};
-      if (head < p.heads && real[j]) {
-        raw0[h][j] = load_values<V>(x + head * p.x_head + at0[j]);
-        raw1[h][j] = load_values<V>(x + head * p.x_head + at1[j]);
+      for (int j = 0; j < K; j++) {
+        if (!rotated[j]) continue;
+        if (PAIRS_IN_PIECES) axes0[j] = axes_of_pairs<V / 2 + (V == 1)>(a, at0[j] / 2), axes1[j] = axes_of_pairs<V / 2 + (V == 1)>(a, at1[j] / 2);
+        else axes0[j] = axes_of_pairs<V>(a, ADJACENT ? at0[j] / 2 : at0[j]);
       }
     }
   }
-  float c[K][V], s[K][V], w0[K][V], w1[K][V];
+  if (kind != HEADS_TO_NONE) slot_index = load_index(a.slots, (int64_t)token * a.slot_stride, a.slots_are_i64);
+
+  typename Piece<V>::type raw0[HEADS][K], raw1[HEADS][K];
+  const u16* x = p.x + (int64_t)token * p.x_token + first_head * p.x_head;
+  const int64_t x_step = per_token * p.x_head;
 #pragma unroll
-  for (int j = 0; j < K; j++) {
+  for (int h = 0; h < HEADS; h++) {
 #pragma unroll
-    for (int i = 0; i < V; i++) w0[j][i] = w1[j][i] = 1.f;
-    if (rotated[j]) load_turn<T, V>(a, pos, (lane + (j << p.lanes_log2)) * V, c[j], s[j]);
-    if (p.w && real[j]) {
-      load_mixed<T, V>(p.w, at0[j], p.w_is_f32, w0[j]);
-      load_mixed<T, V>(p.w, at1[j], p.w_is_f32, w1[j]);
+    for (int j = 0; j < K; j++) {
+      raw0[h][j] = load_values<V>(x + at0[j]);
+      raw1[h][j] = load_values<V>(x + at1[j]);
     }
+    x += first_head + (h + 1) * per_token < heads ? x_step : 0;
   }
 
-  const bool kept = (uint64_t)slot < (uint64_t)a.num_slots;  // (a negative slot is padding)
-  uint32_t page = 0, in_page = 0;
-  if (kept) {
-    page = a.page_div.divide((uint32_t)slot);
-    in_page = (uint32_t)slot - page * (uint32_t)a.page_size;
+  float c[K][V], s[K][V];
+  if (rot_units) {
+    uint32_t table_row[AXES ? 4 : 1];
+    bool inside[AXES ? 4 : 1];
+#pragma unroll
+    for (int k = 0; k < (AXES ? 4 : 1); k++) {
+      const int64_t v = pos[k].value(a.positions_are_i64);
+      inside[k] = (uint64_t)v < (uint64_t)a.table_rows;
+      table_row[k] = inside[k] ? (uint32_t)v * (uint32_t)(a.table_stride * (a.table_is_f32 ? 4 : 2)) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+      if (!rotated[j]) continue;
+      if constexpr (PAIRS_IN_PIECES) {
+        load_turn<T, V / 2, AXES>(a, table_row, inside, axes0[j], at0[j] / 2, c[j], s[j]);
+        load_turn<T, V / 2, AXES>(a, table_row, inside, axes1[j], at1[j] / 2, c[j] + V / 2, s[j] + V / 2);
+      } else {
+        load_turn<T, V, AXES>(a, table_row, inside, axes0[j], ADJACENT ? at0[j] / 2 : at0[j], c[j], s[j]);
+      }
+    }
+  }
+  typename Piece<V>::type raw_w0[K], raw_w1[K];
+  if (NORM && p.w && !p.w_is_f32) {
+#pragma unroll
+    for (int j = 0; j < K; j++) {
+      raw_w0[j] = load_values<V>((const u16*)((const char*)p.w + (uint32_t)(2 * at0[j])));
+      raw_w1[j] = load_values<V>((const u16*)((const char*)p.w + (uint32_t)(2 * at1[j])));
+    }
+  }
+  uint32_t slot = ~0u;
+  if (kind != HEADS_TO_NONE) {
+    const int64_t wide = slot_index.value(a.slots_are_i64);
+    slot = (uint64_t)wide < (uint64_t)a.num_slots ? (uint32_t)wide : ~0u;  // (a negative slot is padding)
   }
 
 #pragma unroll
   for (int h = 0; h < HEADS; h++) {
-    const int head = first_head + h * p.per_token;
-    if (head >= p.heads) return;
+    const int head = first_head + h * per_token;
+    if (head >= heads) return;
+    if (HEADS > 1) __builtin_amdgcn_sched_barrier(0);  // (heads side by side would not fit the registers)
     float f0[K][V], f1[K][V];
 #pragma unroll
     for (int j = 0; j < K; j++) {
-      to_floats<T>(raw0[h][j], f0[j]);
-      to_floats<T>(raw1[h][j], f1[j]);
+      to_floats<T, V>(raw0[h][j], f0[j]);
+      to_floats<T, V>(raw1[h][j], f1[j]);
     }
-    if (p.w) {
-      float sum = 0.f;
+    if constexpr (NORM) {
+      float r = 1.f;
+      if (p.w) {
+        float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < K; j++)
+        for (int j = 0; j < K; j++)
 #pragma unroll
-        for (int i = 0; i < V; i++) sum = fmaf(f0[j][i], f0[j][i], fmaf(f1[j][i], f1[j][i], sum));
-      sum = group_sum(sum, p.lanes_log2);
-      // (a sum beyond fp32 would give zeros)
-      const float r = sum < INFINITY ? rsqrtf(fmaf(sum, p.inv_dim, p.eps)) : NAN;
+          for (int i = 0; i < V; i++) {
+            const float x0 = K == 1 || real[j] ? f0[j][i] : 0.f, x1 = K == 1 || real[j] ? f1[j][i] : 0.f;
+            sum = fmaf(x0, x0, fmaf(x1, x1, sum));
+          }
+        if (K == 1 && !real[0]) sum = 0.f;
+        sum = group_sum(sum, lanes_log2);
+        // (a sum beyond fp32 would give zeros)
+        r = sum < INFINITY ? rsqrtf(fmaf(sum, p.inv_dim, p.eps)) : NAN;
+      }
+      // heads of a part without a weight are multiplied by ones: no second copy of the registers
 #pragma unroll
-      for (int j = 0; j < K; j++)
+      for (int j = 0; j < K; j++) {
+        float w[V];
+        weights<T, V>(p, at0[j], raw_w0[j], w);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          f0[j][i] = f0[j][i] * r * w0[j][i];
-          f1[j][i] = f1[j][i] * r * w1[j][i];
-        }
+        for (int i = 0; i < V; i++) f0[j][i] = f0[j][i] * r * w[i];
+        pin<V>(f0[j]);
+        weights<T, V>(p, at1[j], raw_w1[j], w);
+#pragma unroll
+        for (int i = 0; i < V; i++) f1[j][i] = f1[j][i] * r * w[i];
+        pin<V>(f1[j]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < K; j++)
       if (rotated[j]) turn<V, ADJACENT>(f0[j], f1[j], c[j], s[j]);
 
     if (p.out) {
-      u16* out = p.out + (int64_t)token * p.out_token + head * p.out_head;
+      u16* const out = p.out + (int64_t)token * p.out_token + head * p.out_head;
 #pragma unroll
       for (int j = 0; j < K; j++)
         if (real[j]) {
@@ -315,9 +447,10 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const HeadArgs a) {
           store_values<T, V>(out + at1[j], f1[j]);
         }
     }
-    if (p.kind == HEADS_TO_NONE || !kept) continue;
-    uint8_t* row = p.cache + page * p.cache_page + in_page * p.cache_slot + head * p.cache_head;
-    if (p.kind == HEADS_TO_16) {
+    if (kind == HEADS_TO_NONE || slot == ~0u) continue;
+    const uint32_t page = a.page_div.divide(slot), in_page = slot - page * (uint32_t)a.page_size;
+    uint8_t* const row = p.cache + page * p.cache_page + in_page * p.cache_slot + head * p.cache_head;
+    if (kind == HEADS_TO_16) {
 #pragma unroll
       for (int j = 0; j < K; j++)
         if (real[j]) {
@@ -326,12 +459,9 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const HeadArgs a) {
         }
       continue;
     }
-    // one scale per row, or per 128 values of it
-    uint32_t hi[K], whole = 0;
-    RowScale given = {};
-    if (p.given) {
-      given.mul = fp8_row_multiplier(1.0f, p.given[head * p.given_head]);
-    } else {
+    uint32_t hi[K];
+    if (!p.given) {
+      uint32_t whole = 0;
 #pragma unroll
       for (int j = 0; j < K; j++) {
         hi[j] = 0;
@@ -340,30 +470,26 @@ __global__ __launch_bounds__(256) void head_rows_kernel(const HeadArgs a) {
           hi[j] = umax(hi[j], __float_as_uint(f0[j][i]) & 0x7fffffffu);
           hi[j] = umax(hi[j], __float_as_uint(f1[j][i]) & 0x7fffffffu);
         }
-        if (!real[j]) hi[j] = 0;  // (a row of NaN: its idle lanes' zeros are NaN too)
+        if (!real[j]) hi[j] = 0;
         whole = umax(whole, hi[j]);
       }
-      if (K == 1 || p.scale_units == p.units) {
-        whole = group_umax(whole, p.scale_lanes_log2);
+      if (!p.grouped) whole = group_umax(whole, lanes_log2);
 #pragma unroll
-        for (int j = 0; j < K; j++) hi[j] = whole;
-      } else {
-#pragma unroll
-        for (int j = 0; j < K; j++) hi[j] = group_umax(hi[j], p.scale_lanes_log2);
-      }
+      for (int j = 0; j < K; j++) hi[j] = p.grouped ? group_umax(hi[j], GROUP_LOG2) : whole;
     }
 #pragma unroll
     for (int j = 0; j < K; j++) {
       if (!real[j]) continue;
-      RowScale o = given;
-      if (!p.given) {
-        o = p.kind == HEADS_TO_FP8 ? found_scale<ROW_TO_FP8>(hi[j]) : found_scale<ROW_TO_INT8>(hi[j]);
-        const int u = lane + (j << p.lanes_log2);
-        const int n = p.scale_units == p.units ? 0 : u >> p.scale_lanes_log2;
-        if (u == n * p.scale_units)
+      RowScale o = {};
+      if (p.given) {
+        o.mul = fp8_row_multiplier(1.0f, p.given[head * p.given_head]);
+      } else {
+        o = kind == HEADS_TO_FP8 ? found_scale<ROW_TO_FP8>(hi[j]) : found_scale<ROW_TO_INT8>(hi[j]);
+        const int u = lane + (j << lanes_log2), n = p.grouped ? u >> GROUP_LOG2 : 0;
+        if (u == n << GROUP_LOG2)
           p.scales[page * p.scales_page + in_page * p.scales_slot + head * p.scales_head + n * p.scales_group] = o.scale;
       }
-      if (p.kind == HEADS_TO_FP8) {
+      if (kind == HEADS_TO_FP8) {
         store_codes<ROW_TO_FP8, V>(row + at0[j], f0[j], o);
         store_codes<ROW_TO_FP8, V>(row + at1[j], f1[j], o);
       } else {
@@ -407,6 +533,7 @@ struct Bytes {
 
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
+  touch_arguments(a);
   const int index = a.parts > 1 && blockIdx.x >= a.part[1].first_block;
   const GatherPart& p = a.part[index];
   const uint32_t base = (blockIdx.x - p.first_block) * (256 * GATHER_UNITS) + threadIdx.x;
@@ -419,14 +546,14 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
     const uint32_t in_row = i - row[k] * (uint32_t)p.per_row;
     head[k] = p.per_head_div.divide(in_row);
     unit[k] = in_row - head[k] * (uint32_t)p.per_head;
-    slot[k] = i < p.units ? load_index(a.slots, (int64_t)row[k] * a.slot_stride, a.slots_are_i64) : -1;
+    slot[k] = i < p.units ? load_index(a.slots, (int64_t)row[k] * a.slot_stride, a.slots_are_i64).value(a.slots_are_i64) : -1;
   }
   Bytes<V> codes[GATHER_UNITS];
-  Piece<V> values[GATHER_UNITS];
+  typename Piece<V>::type values[GATHER_UNITS];
   float scale[GATHER_UNITS];
 #pragma unroll
   for (int k = 0; k < GATHER_UNITS; k++) {
-    codes[k] = {}, values[k] = {}, scale[k] = 0.f;
+    codes[k] = {}, values[k] = 0, scale[k] = 0.f;
     if ((uint64_t)slot[k] < (uint64_t)a.num_slots) {
       const uint32_t page = a.page_div.divide((uint32_t)slot[k]), in_page = (uint32_t)slot[k] - page * (uint32_t)a.page_size;
       const uint8_t* src = p.cache + page * p.cache_page + in_page * p.cache_slot + head[k] * p.cache_head;
@@ -445,7 +572,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
     if (base + 256 * k >= p.units) return;
     u16* out = p.out + (int64_t)row[k] * p.out_row + head[k] * p.out_head + unit[k] * V;
     if (p.kind == HEADS_TO_16) {
-      __builtin_memcpy(out, &values[k], 2 * V);
+      __builtin_memcpy(out, &values[k], 2 * V);  // (one value: the low half)
       continue;
     }
     float f[V];
@@ -503,14 +630,19 @@ static int log2_up(int64_t n) {
   return log;
 }
 
-template <typename T, int V, int K, int HEADS>
+template <typename T, int V, int K, int HEADS, bool AXES, bool NORM>
 static void launch_heads(const HeadArgs& a, unsigned blocks, bool adjacent, hipStream_t st) {
-  if (adjacent) hipLaunchKernelGGL((head_rows_kernel<T, V, K, HEADS, true>), dim3(blocks), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((head_rows_kernel<T, V, K, HEADS, false>), dim3(blocks), dim3(256), 0, st, a);
+  if (adjacent) hipLaunchKernelGGL((head_rows_kernel<T, V, K, HEADS, true, AXES, NORM>), dim3(blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((head_rows_kernel<T, V, K, HEADS, false, AXES, NORM>), dim3(blocks), dim3(256), 0, st, a);
+}
+template <typename T, int HEADS, bool AXES>
+static void launch_heads_of_8(const HeadArgs& a, unsigned blocks, bool adjacent, bool norm, hipStream_t st) {
+  if (norm) launch_heads<T, 8, 1, HEADS, AXES, true>(a, blocks, adjacent, st);
+  else launch_heads<T, 8, 1, HEADS, AXES, false>(a, blocks, adjacent, st);
 }
 
-// How many heads of a token a lane group takes.
-constexpr int HEADS_MANY = 4;
+// How many heads of a token a lane group takes where it has to find its cosines pair by pair.
+constexpr int HEADS_MANY = 2;
 
 extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_t tokens, int dtype, const sglamd_rotation* rotation,
                                 const sglamd_slots* slots, void* stream) {
@@ -519,13 +651,15 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   SGLAMD_REQUIRE(dtype == SGLAMD_BF16 || dtype == SGLAMD_F16, SGLAMD_EINVAL, "%s: heads must be Half or BFloat16", op);
   SGLAMD_REQUIRE(tokens >= 0 && tokens < (1ll << 31), SGLAMD_EINVAL, "%s: bad token count %lld", op, (long long)tokens);
   HeadArgs a = {};
-  a.parts = num_parts;
   int64_t width = 0;  // of the rotated part
-  for (int i = 0; i < num_parts; i++)
+  bool norm = false;
+  for (int i = 0; i < num_parts; i++) {
+    norm = norm || parts[i].weight;
     if (parts[i].rotate) {
       SGLAMD_REQUIRE(rotation, SGLAMD_EINVAL, "%s: a rotation without its table", op);
       width = rotation->width;
     }
+  }
   if (width || rotation) {
     const sglamd_rotation& r = *rotation;
     width = r.width;
@@ -534,33 +668,31 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
     SGLAMD_REQUIRE(r.positions_dtype == SGLAMD_I32 || r.positions_dtype == SGLAMD_I64, SGLAMD_EINVAL, "%s: positions must be I32 or I64", op);
     SGLAMD_REQUIRE(r.width > 0 && r.width % 2 == 0 && r.width <= 1024, SGLAMD_EINVAL, "%s: a rotated width of %lld: even, 2 to 1024", op,
                    (long long)r.width);
-    SGLAMD_REQUIRE(r.table_rows >= 0 && r.table_rows < (1ll << 40) && (r.table_rows <= 1 || r.table_stride >= 0), SGLAMD_EINVAL,
-                   "%s: bad table rows or stride", op);
+    SGLAMD_REQUIRE(r.table_rows > 0 && r.table_rows < (1ll << 31) && r.table_stride >= 0 &&
+                       (r.table_rows - 1) * r.table_stride + r.width < (1ll << (r.table_dtype == SGLAMD_F32 ? 29 : 30)),
+                   SGLAMD_EINVAL, "%s: a table of %lld positions: one to 2 GiB are served", op, (long long)r.table_rows);
     SGLAMD_REQUIRE(r.axes >= 1 && r.axes <= 4, SGLAMD_EINVAL, "%s: one to four position axes", op);
     a.table = r.cos_sin, a.table_stride = r.table_stride, a.table_rows = r.table_rows, a.table_is_f32 = r.table_dtype == SGLAMD_F32;
     a.positions = r.positions, a.positions_are_i64 = r.positions_dtype == SGLAMD_I64;
     a.axis_stride = r.axis_stride, a.position_stride = r.position_stride;
-    a.pairs = (int)(r.width / 2), a.axes = r.axes, a.alternating = r.alternating && r.axes > 1;
+    a.pairs = (int)(r.width / 2), a.axes = r.axes;
     if (r.axes > 1) {
-      int64_t sum = 0;
+      int64_t sum = 0, past[4];  // past[k]: behind the last pair of axis k
       for (int k = 0; k < r.axes; k++) {
         SGLAMD_REQUIRE(r.sections[k] >= 0, SGLAMD_EINVAL, "%s: a section is negative", op);
         sum += r.sections[k];
+        past[k] = r.alternating ? (int64_t)r.axes * r.sections[k] : sum;
+        // (the pairs that the rule leaves to axis 0 beyond its own turns have to be as many as its section says)
+        SGLAMD_REQUIRE(!r.alternating || k == 0 || r.sections[k] == 0 || k + (int64_t)r.axes * (r.sections[k] - 1) < a.pairs, SGLAMD_EINVAL,
+                       "%s: alternating sections: axis %d has no %d turns in %d pairs", op, k, (int)r.sections[k], a.pairs);
       }
       SGLAMD_REQUIRE(sum == a.pairs, SGLAMD_EINVAL, "%s: sections of %lld pairs for a rotated width of %lld", op, (long long)sum, (long long)r.width);
-      if (a.alternating) {
-        a.axis_inv = (65536 + r.axes - 1) / r.axes;
-        for (int k = 0; k < 4; k++) a.section[k] = k < r.axes ? r.sections[k] : 0;
-        // the pairs that the rule gives to axis 0 beyond its own turns have to be as many as its section says
-        for (int k = 1; k < r.axes; k++)
-          SGLAMD_REQUIRE(r.sections[k] == 0 || k + (int64_t)r.axes * (r.sections[k] - 1) < a.pairs, SGLAMD_EINVAL,
-                         "%s: alternating sections: axis %d has no %d turns in %d pairs", op, k, (int)r.sections[k], a.pairs);
-      } else {
-        int at = 0;
-        for (int k = 0; k < 4; k++) {  // where axis k begins (axes that are not there: behind the last pair)
-          a.section[k] = k < r.axes ? at : a.pairs;
-          if (k < r.axes) at += r.sections[k];
-        }
+      for (int i = 0; i < a.pairs; i++) {
+        int k = 0;
+        if (r.alternating) k = i < past[i % r.axes] ? i % r.axes : 0;
+        else while (i >= past[k]) k++;
+        a.axis_bits[0][i / 32] |= (uint32_t)(k & 1) << (i % 32);
+        a.axis_bits[1][i / 32] |= (uint32_t)(k >> 1) << (i % 32);
       }
     }
   }
@@ -585,10 +717,13 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
     if (v == 4 && parts[i].dim > 512) v = 1;
   const int k = v == 1 ? 8 : 1;
 
-  // one head per lane group until the heads of a launch fill the chip
+  // One head per lane group: 57 to 64 registers, eight waves a SIMD, and the most loads in flight (8191 tokens of 64 + 2 x 8 heads
+  // of 128 into e4m3 rows: 62 us, two heads 64, four 67).  With several axes a lane may need sixteen loads for its pairs, which
+  // two heads share once there are enough of them to fill half of the chip (2901 tokens of 32 heads, alternating axes: 13.0 us, one
+  // head 15.8, four 12.2; 4096 of 72, normalised: 38.5, 44.2, 37.4; blocks of axes: 35.8, 37.4, 36.5).
   int64_t lanes = 0;
   for (int i = 0; i < num_parts; i++) lanes += tokens * parts[i].heads << log2_up(ceil_div(parts[i].dim, 2 * v * k));
-  const int many = v == 8 && lanes >= (int64_t)device_cus() * 2048 * 4 ? HEADS_MANY : 1;
+  const int many = v == 8 && a.axes > 1 && lanes >= (int64_t)device_cus() * 1024 ? HEADS_MANY : 1;
 
   uint64_t blocks = 0;
   for (int i = 0; i < num_parts; i++) {
@@ -601,7 +736,7 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
                    "%s: a norm weight must be Float or of the heads' type", op);
     SGLAMD_REQUIRE(!h.weight || (h.eps >= 0.f && h.eps < INFINITY), SGLAMD_EINVAL, "%s: epsilon must be finite and not negative", op);
     p.x = (const u16*)h.x, p.x_token = h.x_token, p.x_head = h.x_head;
-    p.w = h.weight, p.w_is_f32 = h.weight_dtype == SGLAMD_F32, p.eps = h.eps, p.inv_dim = 1.0f / (float)h.dim;
+    p.w = h.weight, p.w_is_f32 = h.weight && h.weight_dtype == SGLAMD_F32, p.eps = h.eps, p.inv_dim = 1.0f / (float)h.dim;
     p.out = (u16*)h.out, p.out_token = h.out_token, p.out_head = h.out_head;
     p.heads = (int)h.heads, p.units = (int)(h.dim / (2 * v)), p.rot_units = h.rotate ? (int)(width / (2 * v)) : 0;
     p.lanes_log2 = log2_up(ceil_div(p.units, k));
@@ -614,11 +749,10 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
       p.cache = (uint8_t*)h.cache, p.cache_page = h.cache_page * bytes, p.cache_slot = h.cache_slot * bytes, p.cache_head = h.cache_head * bytes;
       p.given = h.given_scale, p.given_head = h.given_head, p.scales = h.scales;
       p.scales_page = h.scales_page, p.scales_slot = h.scales_slot, p.scales_head = h.scales_head, p.scales_group = h.scales_group;
-      p.scale_units = p.units, p.scale_lanes_log2 = p.lanes_log2;
       if (h.scales && h.scale_group != h.dim) {
         SGLAMD_REQUIRE(h.scale_group == 128 && h.dim % 128 == 0 && !h.rotate, SGLAMD_EINVAL,
                        "%s: a scale per row, or per 128 values of rows that are not rotated and a multiple of 128 long", op);
-        p.scale_units = 64 / v, p.scale_lanes_log2 = log2_up(p.scale_units);
+        p.grouped = 1;
         if (k > 1) p.lanes_log2 = 6;  // a round of the wave's lanes is one scale
       }
     }
@@ -627,9 +761,10 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
     SGLAMD_REQUIRE(groups << p.lanes_log2 < (1ull << 31), SGLAMD_EINVAL, "%s: %lld tokens of %lld heads are too many for one launch", op,
                    (long long)tokens, (long long)h.heads);
     p.groups = (uint32_t)groups, p.per_token_div = FastDiv::of((uint32_t)(p.per_token ? p.per_token : 1));
-    p.first_block = (uint32_t)blocks;
+    a.first_block[i] = (uint32_t)blocks;
     blocks += ((groups << p.lanes_log2) + 255) / 256;
   }
+  for (int i = num_parts; i < MAX_PARTS; i++) a.first_block[i] = ~0u;
   if (blocks == 0) return SGLAMD_OK;
   SGLAMD_REQUIRE(blocks < (1ull << 24), SGLAMD_EINVAL, "%s: %lld tokens are too many for one launch", op, (long long)tokens);
   const bool adjacent = rotation && rotation->interleaved;
@@ -637,10 +772,11 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   const DeviceScope scope;
 #define SGLAMD_HEADS(T)                                                                       \
   do {                                                                                        \
-    if (v == 8 && many > 1) launch_heads<T, 8, 1, HEADS_MANY>(a, (unsigned)blocks, adjacent, st); \
-    else if (v == 8) launch_heads<T, 8, 1, 1>(a, (unsigned)blocks, adjacent, st);             \
-    else if (v == 4) launch_heads<T, 4, 1, 1>(a, (unsigned)blocks, adjacent, st);             \
-    else launch_heads<T, 1, 8, 1>(a, (unsigned)blocks, adjacent, st);                         \
+    if (v == 8 && many > 1) launch_heads_of_8<T, HEADS_MANY, true>(a, (unsigned)blocks, adjacent, norm, st); \
+    else if (v == 8 && a.axes > 1) launch_heads_of_8<T, 1, true>(a, (unsigned)blocks, adjacent, norm, st);   \
+    else if (v == 8) launch_heads_of_8<T, 1, false>(a, (unsigned)blocks, adjacent, norm, st);                \
+    else if (v == 4) launch_heads<T, 4, 1, 1, true, true>(a, (unsigned)blocks, adjacent, st); \
+    else launch_heads<T, 1, 8, 1, true, true>(a, (unsigned)blocks, adjacent, st);             \
   } while (0)
   if (dtype == SGLAMD_BF16) SGLAMD_HEADS(BF16);
   else SGLAMD_HEADS(F16);
@@ -659,14 +795,14 @@ extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts
   GatherArgs a = {};
   a.parts = num_parts, a.slots = slots->slots, a.slot_stride = slots->slot_stride, a.slots_are_i64 = slots->slots_dtype == SGLAMD_I64;
   a.num_slots = slots->page_size * slots->pages, a.page_size = (int)slots->page_size, a.page_div = FastDiv::of((uint32_t)slots->page_size);
-  int v = 16;
+  int v = 8;
   for (int i = 0; i < num_parts; i++) {
     const sglamd_gather& g = parts[i];
     SGLAMD_REQUIRE(g.heads >= 0 && g.heads < (1 << 20) && g.dim > 0 && g.dim <= 1024, SGLAMD_EINVAL, "%s: %lld heads of %lld values: up to 1024", op,
                    (long long)g.heads, (long long)g.dim);
     while (v > 1 && g.dim % v) v /= 2;
   }
-  if (v < 8) v = v == 4 ? 4 : 1;
+  if (v == 2) v = 1;
   uint64_t blocks = 0;
   for (int i = 0; i < num_parts; i++) {
     const sglamd_gather& g = parts[i];
@@ -695,8 +831,7 @@ extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts
   hipStream_t st = (hipStream_t)stream;
 #define SGLAMD_GATHER(T)                                                                                                       \
   do {                                                                                                                         \
-    if (v == 16) hipLaunchKernelGGL((gather_rows_kernel<T, 16>), dim3((unsigned)blocks), dim3(256), 0, st, a);                 \
-    else if (v == 8) hipLaunchKernelGGL((gather_rows_kernel<T, 8>), dim3((unsigned)blocks), dim3(256), 0, st, a);              \
+    if (v == 8) hipLaunchKernelGGL((gather_rows_kernel<T, 8>), dim3((unsigned)blocks), dim3(256), 0, st, a);              \
     else if (v == 4) hipLaunchKernelGGL((gather_rows_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);              \
     else hipLaunchKernelGGL((gather_rows_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);                          \
   } while (0)

@@ -604,7 +604,7 @@ struct HeadsCall {
   // The rotation by a table of `cos_sin.size(1)` cosines and sines.
   void rotate_by(const Tensor& positions, const Tensor& cos_sin, bool interleaved, const optional<std::vector<int64_t>>& sections, bool alternating,
                  int64_t tokens, ScalarType type) {
-    TORCH_CHECK(cos_sin.dim() == 2, "cos_sin must be [positions, rotated width]");
+    TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(0) > 0, "cos_sin must be [positions, rotated width], at least one position");
     const int64_t width = cos_sin.size(1);
     TORCH_CHECK(width > 0 && width % 2 == 0 && width <= 1024, "cos_sin: a rotated width of ", width, ": even, 2 to 1024");
     TORCH_CHECK(cos_sin.stride(1) == 1, "cos_sin rows must be contiguous");

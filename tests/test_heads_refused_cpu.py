@@ -36,6 +36,7 @@ ROTATE = [
     ("positions must be \\[tokens\\]", dict(positions=torch.zeros(3, T, dtype=torch.long))),
     ("positions must be Int or Long", dict(positions=torch.zeros(T))),
     ("cos_sin must be \\[positions", dict(cos_sin=Z(64))),
+    ("at least one position", dict(cos_sin=Z(0, 64, dtype=torch.float32))),
     ("even, 2 to 1024", dict(cos_sin=Z(10, 63, dtype=torch.float32))),
     ("a rotated width of 66 for q of 64", dict(cos_sin=Z(10, 66, dtype=torch.float32))),
     ("cos_sin must be Float32", dict(cos_sin=Z(10, 64, dtype=torch.float16))),
@@ -253,6 +254,7 @@ def test_c_interface_refuses_before_any_launch():
             (b"without its table", 1, 2, heads(rotate=1), None, None),
             (b"even, 2 to 1024", 1, 2, heads(rotate=1), rotation(width=0), None),
             (b"a rotated width of 128 in heads of 64", 1, 2, heads(rotate=1), rotation(width=128), None),
+            (b"a table of 0 positions", 1, 2, heads(rotate=1), rotation(table_rows=0), None),
             (b"null table", 1, 2, heads(rotate=1), rotation(positions=None), None),
             (b"positions must be", 1, 2, heads(rotate=1), rotation(positions_dtype=0), None),
             (b"the table must be", 1, 2, heads(rotate=1), rotation(table_dtype=1), None),
