@@ -103,14 +103,21 @@ __device__ __forceinline__ void to_floats(const typename Piece<V>::type& p, floa
     for (int i = 0; i < V / 2; i++) f[2 * i] = T::to_f32((u16)p[i]), f[2 * i + 1] = T::to_f32((u16)(p[i] >> 16));
   }
 }
+// The last product of a value is rounded to fp32 before its conversion: one instruction makes both for halves and rounds once, and
+// the compiler takes it for some values of a row and not for others, so that a row's last bits would depend on the instance.
+template <typename T>
+__device__ __forceinline__ float in_fp32(float f) {
+  if constexpr (T::tag == SGLAMD_F16) asm("" : "+v"(f));
+  return f;
+}
 template <typename T, int V>
 __device__ __forceinline__ void store_values(u16* p, const float* f) {
   if constexpr (V == 1) {
-    *p = T::from_f32(f[0]);
+    *p = T::from_f32(in_fp32<T>(f[0]));
   } else {
     uint32_t w[V / 2];
 #pragma unroll
-    for (int i = 0; i < V / 2; i++) w[i] = T::pack2(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < V / 2; i++) w[i] = T::pack2(in_fp32<T>(f[2 * i]), in_fp32<T>(f[2 * i + 1]));
     __builtin_memcpy(p, w, 2 * V);
   }
 }
@@ -524,54 +531,59 @@ struct GatherArgs {
   FastDiv page_div;
 };
 
-constexpr int GATHER_UNITS = 4;  // a lane's units: their loads are in flight together
-
 template <int V>
 struct Bytes {
   uint8_t v[V];
 };
 
-template <typename T, int V>
+// A lane takes UNITS units of V values, 256 units apart.  The slots of all of them are asked for first, then the rows without a
+// condition (where there is no slot, those of slot 0): two round trips, whatever UNITS.  Pieces of eight values, not sixteen: stores
+// of 16 bytes beside each other (65000 int8 rows of 2 x 8 x 128: 80 us, a copy of as much 80; sixteen 95).
+template <typename T, int V, int UNITS>
 __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
   touch_arguments(a);
   const int index = a.parts > 1 && blockIdx.x >= a.part[1].first_block;
   const GatherPart& p = a.part[index];
-  const uint32_t base = (blockIdx.x - p.first_block) * (256 * GATHER_UNITS) + threadIdx.x;
-  uint32_t row[GATHER_UNITS], head[GATHER_UNITS], unit[GATHER_UNITS];
-  int64_t slot[GATHER_UNITS];
+  const uint32_t base = (blockIdx.x - p.first_block) * (256 * UNITS) + threadIdx.x;
+  uint32_t row[UNITS], head[UNITS], unit[UNITS];
+  Index slot_index[UNITS];
 #pragma unroll
-  for (int k = 0; k < GATHER_UNITS; k++) {
-    const uint32_t i = base + 256 * k;
+  for (int k = 0; k < UNITS; k++) {
+    const uint32_t i = min(base + 256 * k, p.units - 1);  // (lanes and units that are none read the last one)
     row[k] = p.per_row_div.divide(i);
     const uint32_t in_row = i - row[k] * (uint32_t)p.per_row;
     head[k] = p.per_head_div.divide(in_row);
     unit[k] = in_row - head[k] * (uint32_t)p.per_head;
-    slot[k] = i < p.units ? load_index(a.slots, (int64_t)row[k] * a.slot_stride, a.slots_are_i64).value(a.slots_are_i64) : -1;
+    slot_index[k] = load_index(a.slots, (int64_t)row[k] * a.slot_stride, a.slots_are_i64);
   }
-  Bytes<V> codes[GATHER_UNITS];
-  typename Piece<V>::type values[GATHER_UNITS];
-  float scale[GATHER_UNITS];
+  Bytes<V> codes[UNITS] = {};
+  typename Piece<V>::type values[UNITS];
+  float scale[UNITS] = {};
+  bool inside[UNITS];
 #pragma unroll
-  for (int k = 0; k < GATHER_UNITS; k++) {
-    codes[k] = {}, values[k] = 0, scale[k] = 0.f;
-    if ((uint64_t)slot[k] < (uint64_t)a.num_slots) {
-      const uint32_t page = a.page_div.divide((uint32_t)slot[k]), in_page = (uint32_t)slot[k] - page * (uint32_t)a.page_size;
-      const uint8_t* src = p.cache + page * p.cache_page + in_page * p.cache_slot + head[k] * p.cache_head;
-      if (p.kind == HEADS_TO_16) {
-        values[k] = load_values<V>((const u16*)src + unit[k] * V);
-      } else {
-        __builtin_memcpy(&codes[k], src + unit[k] * V, V);
-        scale[k] = p.given ? p.given[head[k] * p.given_head]
-                           : p.scales[page * p.scales_page + in_page * p.scales_slot + head[k] * p.scales_head +
-                                      (unit[k] >> p.group_units_log2) * p.scales_group];
-      }
+  for (int k = 0; k < UNITS; k++) {
+    const int64_t wide = slot_index[k].value(a.slots_are_i64);
+    inside[k] = (uint64_t)wide < (uint64_t)a.num_slots;
+    const uint32_t slot = inside[k] ? (uint32_t)wide : 0;
+    const uint32_t page = a.page_div.divide(slot), in_page = slot - page * (uint32_t)a.page_size;
+    const uint8_t* src = p.cache + page * p.cache_page + in_page * p.cache_slot + head[k] * p.cache_head;
+    values[k] = 0;
+    if (a.num_slots == 0) continue;
+    if (p.kind == HEADS_TO_16) {
+      values[k] = load_values<V>((const u16*)src + unit[k] * V);
+    } else {
+      __builtin_memcpy(&codes[k], src + unit[k] * V, V);
+      scale[k] = p.given ? p.given[head[k] * p.given_head]
+                         : p.scales[page * p.scales_page + in_page * p.scales_slot + head[k] * p.scales_head +
+                                    (unit[k] >> p.group_units_log2) * p.scales_group];
     }
   }
 #pragma unroll
-  for (int k = 0; k < GATHER_UNITS; k++) {
+  for (int k = 0; k < UNITS; k++) {
     if (base + 256 * k >= p.units) return;
     u16* out = p.out + (int64_t)row[k] * p.out_row + head[k] * p.out_head + unit[k] * V;
-    if (p.kind == HEADS_TO_16) {
+    if (p.kind == HEADS_TO_16 || !inside[k]) {
+      if (!inside[k]) values[k] = 0;
       __builtin_memcpy(out, &values[k], 2 * V);  // (one value: the low half)
       continue;
     }
@@ -594,7 +606,6 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const GatherArgs a) {
 #pragma unroll
       for (int i = 0; i < V; i++) f[i] = (float)(int8_t)codes[k].v[i] * scale[k];
     }
-    // (a slot that is none gives zeros, also where a given scale is not finite)
     store_values<T, V>(out, f);
   }
 }
@@ -643,6 +654,8 @@ static void launch_heads_of_8(const HeadArgs& a, unsigned blocks, bool adjacent,
 
 // How many heads of a token a lane group takes where it has to find its cosines pair by pair.
 constexpr int HEADS_MANY = 2;
+// ... and where its pieces are of four values.
+constexpr int HEADS_OF_FOURS = 4;
 
 extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_t tokens, int dtype, const sglamd_rotation* rotation,
                                 const sglamd_slots* slots, void* stream) {
@@ -723,7 +736,11 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   // head 15.8, four 12.2; 4096 of 72, normalised: 38.5, 44.2, 37.4; blocks of axes: 35.8, 37.4, 36.5).
   int64_t lanes = 0;
   for (int i = 0; i < num_parts; i++) lanes += tokens * parts[i].heads << log2_up(ceil_div(parts[i].dim, 2 * v * k));
-  const int many = v == 8 && a.axes > 1 && lanes >= (int64_t)device_cus() * 1024 ? HEADS_MANY : 1;
+  // Pieces of four: the lanes' addresses are most of the work, four heads share them (4096 tokens of 72 heads of 72, normalised: 28 us,
+  // two heads 31, eight 31, one 39; 500 of 80 heads of 72 into e4m3 rows: four 8.3, one 7.0).
+  const DeviceScope scope;
+  const int64_t cus = device_cus();
+  const int many = v == 4 && lanes >= cus * 4096 ? HEADS_OF_FOURS : v == 8 && a.axes > 1 && lanes >= cus * 1024 ? HEADS_MANY : 1;
 
   uint64_t blocks = 0;
   for (int i = 0; i < num_parts; i++) {
@@ -769,19 +786,25 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   SGLAMD_REQUIRE(blocks < (1ull << 24), SGLAMD_EINVAL, "%s: %lld tokens are too many for one launch", op, (long long)tokens);
   const bool adjacent = rotation && rotation->interleaved;
   hipStream_t st = (hipStream_t)stream;
-  const DeviceScope scope;
 #define SGLAMD_HEADS(T)                                                                       \
   do {                                                                                        \
     if (v == 8 && many > 1) launch_heads_of_8<T, HEADS_MANY, true>(a, (unsigned)blocks, adjacent, norm, st); \
     else if (v == 8 && a.axes > 1) launch_heads_of_8<T, 1, true>(a, (unsigned)blocks, adjacent, norm, st);   \
     else if (v == 8) launch_heads_of_8<T, 1, false>(a, (unsigned)blocks, adjacent, norm, st);                \
-    else if (v == 4) launch_heads<T, 4, 1, 1, true, true>(a, (unsigned)blocks, adjacent, st); \
+    else if (v == 4 && many > 1) launch_heads<T, 4, 1, HEADS_OF_FOURS, true, true>(a, (unsigned)blocks, adjacent, st); \
+    else if (v == 4) launch_heads<T, 4, 1, 1, true, true>(a, (unsigned)blocks, adjacent, st);                    \
     else launch_heads<T, 1, 8, 1, true, true>(a, (unsigned)blocks, adjacent, st);             \
   } while (0)
   if (dtype == SGLAMD_BF16) SGLAMD_HEADS(BF16);
   else SGLAMD_HEADS(F16);
 #undef SGLAMD_HEADS
   return check_launch(op);
+}
+
+template <typename T, int V>
+static void launch_gather(const GatherArgs& a, unsigned blocks, int per_lane, hipStream_t st) {
+  if (per_lane == 4) hipLaunchKernelGGL((gather_rows_kernel<T, V, 4>), dim3(blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gather_rows_kernel<T, V, 1>), dim3(blocks), dim3(256), 0, st, a);
 }
 
 extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts, int64_t rows, int dtype, const sglamd_slots* slots, void* stream) {
@@ -803,6 +826,12 @@ extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts
     while (v > 1 && g.dim % v) v /= 2;
   }
   if (v == 2) v = 1;
+  // Four units a lane once one each fills the chip several times over (int8 rows of 2 x 8 x 128, one | four: 500 of them 2.7 | 4.2 us,
+  // 10000 13.3 | 15.4, 20000 30.8 | 28.6, 65000 92.8 | 80.9).
+  const DeviceScope scope;
+  int64_t all = 0;
+  for (int i = 0; i < num_parts; i++) all += rows * parts[i].heads * (parts[i].dim / v);
+  const int per_lane = all > (int64_t)device_cus() * 16384 ? 4 : 1;
   uint64_t blocks = 0;
   for (int i = 0; i < num_parts; i++) {
     const sglamd_gather& g = parts[i];
@@ -821,19 +850,19 @@ extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts
     p.out = (u16*)g.out, p.out_row = g.out_row, p.out_head = g.out_head;
     p.per_head = (int)(g.dim / v), p.per_row = p.per_head * (int)g.heads;
     const uint64_t units = (uint64_t)rows * (uint64_t)p.per_row;
-    SGLAMD_REQUIRE((uint64_t)g.heads * (uint64_t)p.per_head < (1ull << 31) && units < (1ull << 31) - 256 * GATHER_UNITS, SGLAMD_EINVAL,
+    SGLAMD_REQUIRE((uint64_t)g.heads * (uint64_t)p.per_head < (1ull << 31) && units < (1ull << 31) - 1024, SGLAMD_EINVAL,
                    "%s: %lld rows are too many for one launch", op, (long long)rows);
     p.units = (uint32_t)units, p.per_row_div = FastDiv::of((uint32_t)(p.per_row ? p.per_row : 1)), p.per_head_div = FastDiv::of((uint32_t)p.per_head);
     p.first_block = (uint32_t)blocks;
-    blocks += (units + 256 * GATHER_UNITS - 1) / (256 * GATHER_UNITS);
+    blocks += (units + 256 * per_lane - 1) / (256 * per_lane);
   }
   if (blocks == 0) return SGLAMD_OK;
   hipStream_t st = (hipStream_t)stream;
-#define SGLAMD_GATHER(T)                                                                                                       \
-  do {                                                                                                                         \
-    if (v == 8) hipLaunchKernelGGL((gather_rows_kernel<T, 8>), dim3((unsigned)blocks), dim3(256), 0, st, a);              \
-    else if (v == 4) hipLaunchKernelGGL((gather_rows_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);              \
-    else hipLaunchKernelGGL((gather_rows_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);                          \
+#define SGLAMD_GATHER(T)                                                       \
+  do {                                                                         \
+    if (v == 8) launch_gather<T, 8>(a, (unsigned)blocks, per_lane, st);        \
+    else if (v == 4) launch_gather<T, 4>(a, (unsigned)blocks, per_lane, st);   \
+    else launch_gather<T, 1>(a, (unsigned)blocks, per_lane, st);               \
   } while (0)
   if (dtype == SGLAMD_BF16) SGLAMD_GATHER(BF16);
   else SGLAMD_GATHER(F16);

@@ -506,10 +506,9 @@ Tensor int8_weight_sums(const Tensor& weight) {
 // ---------------------------------------------------------------------------------------
 // The memory of a tensor, for calls that write into tensors they are given.
 struct Span {
-  const char* name;
   const uint8_t *begin, *end;  // all of it lies in [begin, end)
-  int64_t item, dims = 0, sizes[4] = {}, strides[4] = {};  // bytes; dimensions of more than one element
-  Span(const char* name_, const Tensor& t) : name(name_), begin((const uint8_t*)t.data_ptr()), end(begin), item(t.element_size()) {
+  int64_t item, dims = 0, sizes[4], strides[4];  // bytes; dimensions of more than one element
+  explicit Span(const Tensor& t) : begin((const uint8_t*)t.data_ptr()), end(begin), item(t.element_size()) {
     if (t.numel() == 0) return;
     end += item;
     for (int64_t d = 0; d < t.dim(); d++)
@@ -573,19 +572,23 @@ struct HeadsCall {
   sglamd_rotation rotation = {};
   sglamd_slots slots = {};
   const Tensor* first = nullptr;
-  std::vector<const Tensor*> reads, writes;
-  std::vector<const char*> read_names, write_names;
-  std::vector<std::pair<size_t, size_t>> in_place;  // (read, write) that may be one and the same tensor
+  struct Operand {
+    const Tensor* tensor;
+    const char* name;
+    int from;  // written: the read operand that it may be one and the same tensor with, or -1
+  };
+  Operand reads[16], writes[8];  // (the longest call has 13 and 6)
+  int num_reads = 0, num_writes = 0;
 
   explicit HeadsCall(const char* name) : op(name) {}
 
   void reading(const Tensor& t, const char* name) {
     if (!first) first = &t;
-    reads.push_back(&t), read_names.push_back(name);
+    reads[num_reads++] = {&t, name, -1};
   }
-  void writing(const Tensor& t, const char* name) {
+  void writing(const Tensor& t, const char* name, int from = -1) {
     if (!first) first = &t;
-    writes.push_back(&t), write_names.push_back(name);
+    writes[num_writes++] = {&t, name, from};
   }
 
   static void check_heads(const Tensor& t, const char* name, int64_t tokens, ScalarType type) {
@@ -662,8 +665,7 @@ struct HeadsCall {
     if (!given) return;
     TORCH_CHECK(given->sizes() == x.sizes() && given->scalar_type() == x.scalar_type(), name, " must match its input");
     check_width(*given, name);
-    in_place.push_back({reads.size() - 1, writes.size()});
-    writing(*given, name);
+    writing(*given, name, num_reads - 1);
   }
   static Tensor allocate(const Tensor& x, const optional<Tensor>& given) { return given ? *given : at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous); }
   static void point(sglamd_heads& h, const Tensor& x, const Tensor& out) {
@@ -736,34 +738,30 @@ struct HeadsCall {
   // What the shapes do not say.  There is no torch.ops schema: who has to see an operator is refused.
   void check_tensors() const {
     bool observed = is_observed();
-    for (const auto* list : {&reads, &writes})
-      for (const Tensor* t : *list) observed = observed || (t->is_cuda() && is_observed(*t));
+    for (int i = 0; i < num_reads; i++) observed = observed || (reads[i].tensor->is_cuda() && is_observed(*reads[i].tensor));
+    for (int i = 0; i < num_writes; i++) observed = observed || (writes[i].tensor->is_cuda() && is_observed(*writes[i].tensor));
     if (observed)
       C10_THROW_ERROR(NotImplementedError, std::string(op) + " has no gradient and takes plain tensors only, outside of tracers and "
                                                              "transforms (call it under torch.no_grad())");
-    std::vector<Span> from, to;
-    from.reserve(reads.size()), to.reserve(writes.size());
-    for (size_t i = 0; i < writes.size(); i++) to.emplace_back(write_names[i], *writes[i]);
-    if (!to.empty())
-      for (size_t i = 0; i < reads.size(); i++) from.emplace_back(read_names[i], *reads[i]);
-    for (size_t i = 0; i < to.size(); i++) {
-      TORCH_CHECK(is_apart(to[i]), to[i].name, " must not be expanded or overlap itself");
-      for (size_t j = 0; j < i; j++) TORCH_CHECK(disjoint(to[i], to[j]), to[i].name, " must not overlap ", to[j].name);
-      for (size_t j = 0; j < from.size(); j++) {
-        const bool may = std::find(in_place.begin(), in_place.end(), std::make_pair(j, i)) != in_place.end() && to[i].same(from[j]);
-        TORCH_CHECK(may || disjoint(to[i], from[j]), to[i].name, " must not overlap ", from[j].name);
+    for (int i = 0; i < num_writes; i++) {
+      const Span to(*writes[i].tensor);
+      TORCH_CHECK(is_apart(to), writes[i].name, " must not be expanded or overlap itself");
+      for (int j = 0; j < i; j++) TORCH_CHECK(disjoint(to, Span(*writes[j].tensor)), writes[i].name, " must not overlap ", writes[j].name);
+      for (int j = 0; j < num_reads; j++) {
+        const Span from(*reads[j].tensor);
+        TORCH_CHECK((writes[i].from == j && to.same(from)) || disjoint(to, from), writes[i].name, " must not overlap ", reads[j].name);
       }
     }
-    for (const auto* list : {&reads, &writes})
-      for (const Tensor* t : *list) {
-        TORCH_CHECK(t->is_cuda(), op, ": every tensor must be a CUDA tensor");
-        TORCH_CHECK(t->device() == first->device(), op, ": every tensor must be on the same device");
-      }
+    for (int i = 0; i < num_reads + num_writes; i++) {
+      const Tensor& t = i < num_reads ? *reads[i].tensor : *writes[i - num_reads].tensor;
+      TORCH_CHECK(t.is_cuda(), op, ": every tensor must be a CUDA tensor");
+      TORCH_CHECK(t.device() == first->device(), op, ": every tensor must be on the same device");
+    }
   }
   void launch(int64_t tokens, ScalarType type, bool rotated) {
     if (tokens)
       check(sglamd_head_rows(part, parts, tokens, tag(type), rotated ? &rotation : nullptr, slots.slots ? &slots : nullptr, stream_of(*first)));
-    for (const Tensor* t : writes) written_in_place(*t);
+    for (int i = 0; i < num_writes; i++) written_in_place(*writes[i].tensor);
   }
 };
 
@@ -932,7 +930,7 @@ void gather_into(HeadsCall& call, int64_t rows, ScalarType type, const Tensor& f
     g.out = address(*outs[i]), g.out_row = outs[i]->stride(0), g.out_head = outs[i]->dim() == 2 ? 0 : outs[i]->stride(1);
   }
   if (rows) check(sglamd_gather_head_rows(call.back, 2, rows, tag(type), &call.slots, stream_of(slots)));
-  for (const Tensor* t : call.writes) written_in_place(*t);
+  for (int i = 0; i < call.num_writes; i++) written_in_place(*call.writes[i].tensor);
 }
 
 void check_gather(const Tensor& cache, const char* name, int64_t row_dims, sglamd_gather& g) {

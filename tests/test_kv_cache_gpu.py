@@ -117,7 +117,19 @@ def test_append_forms(dev, dtype, kind):
 
 @pytest.mark.parametrize("kind", KINDS)
 def test_append_many(dev, kind):
-    run_append(4100, 61, 7, 128, 128, 128, kind, 16, norm=kind == "16")
+    run_append(1030, 61, 7, 128, 128, 128, kind, 16, norm=kind == "16")
+    run_append(1030, 61, 7, 72, 72, 72, kind, 16, norm=kind != "16")
+
+
+@pytest.mark.parametrize("kind", ["16", "int8_rows"])
+def test_gather_many(dev, kind):
+    """Launches of four units a lane: 17000 rows of 2 x 8 x 128."""
+    g = torch.Generator().manual_seed(21)
+    caches = [make_cache(g, kind, 100, 16, (8, 128), BF16) for _ in range(2)]
+    slots = torch.randint(-1, 1601, (17000,), generator=g).cuda()
+    got = gather_kv(caches[0][0], caches[1][0], slots, BF16, k_scale=caches[0][1], v_scale=caches[1][1])
+    for rows, (cache, scale) in zip(got, caches):
+        assert torch.equal(rows.cpu(), gathered(cache, scale, slots, BF16, 1600, (8, 128)))
 
 
 def test_keys_and_values_alone(dev):
@@ -357,3 +369,60 @@ def test_latent_rows_of_one_buffer(dev):
     rest = torch.ones(160, dtype=torch.bool, device=dev)
     rest[slots] = False
     assert not raw.view(160, -1)[rest].any()
+
+
+def test_in_place(dev):
+    """Queries and keys rotated in their own buffer, a view of the projection, while they go into the cache."""
+    g = torch.Generator().manual_seed(14)
+    qkv = heads(g, 9, 8, 64, dtype=BF16).cuda()
+    before = qkv.clone()
+    positions, cos_sin, slots = torch.randint(0, 50, (9,), generator=g).cuda(), table(50, 64).cuda(), torch.randperm(20, generator=g)[:9].cuda()
+    caches = [torch.zeros(20, 2, 64, device=dev, dtype=BF16) for _ in range(2)]
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    got = append_kv(k, v, *caches, slots, q=q, positions=positions, cos_sin=cos_sin, q_out=q, k_out=k)
+    assert got[0].data_ptr() == q.data_ptr() and got[1].data_ptr() == k.data_ptr()
+    check_16(q, *turned(*normed(before[:, :4], None, EPS), positions, cos_sin, False))
+    check_16(k, *turned(*normed(before[:, 4:6], None, EPS), positions, cos_sin, False))
+    assert torch.equal(v, before[:, 6:]) and torch.equal(caches[0][slots], k) and torch.equal(caches[1][slots], v)
+
+
+def test_two_streams_into_one_cache(dev):
+    g = torch.Generator().manual_seed(15)
+    k = heads(g, 2, 400, 8, 128, dtype=BF16).cuda()
+    slots = torch.randperm(1000, generator=g)[:800].view(2, 400).cuda()
+    (kc, ks), (vc, vs) = (make_cache(g, "int8_rows", 125, 8, (8, 128), BF16) for _ in range(2))
+    want = [t.clone() for t in (kc, ks, vc, vs)]
+    for i in range(2):
+        append_kv(k[i], k[i], want[0], want[2], slots[i], k_scale=want[1], v_scale=want[3])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            append_kv(k[i], k[i], kc, vc, slots[i], k_scale=ks, v_scale=vs)
+    torch.cuda.synchronize()
+    for got, ref in zip((kc, ks, vc, vs), want):
+        assert torch.equal(got, ref)
+
+
+def test_the_same_slot_twice(dev):
+    """Either of the two rows, or parts of both; all other rows as they were."""
+    k = torch.stack([torch.full((2, 64), 1.0), torch.full((2, 64), 2.0), torch.full((2, 64), 3.0)]).to(BF16).cuda()
+    cache = torch.zeros(6, 2, 64, device=dev, dtype=BF16)
+    append_kv(k, k, cache, torch.zeros_like(cache), torch.tensor([4, 1, 4], device=dev))
+    assert ((cache[4] == 1) | (cache[4] == 3)).all() and (cache[1] == 2).all() and not cache[[0, 2, 3, 5]].any()
+
+
+def test_gradients_are_refused(dev):
+    leaf = torch.ones(3, 2, 64, device=dev, dtype=BF16, requires_grad=True)
+    x, cache, slots = torch.ones(3, 2, 64, device=dev, dtype=BF16), torch.zeros(6, 2, 64, device=dev, dtype=BF16), torch.arange(3, device=dev)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        append_kv(leaf, x, cache, cache.clone(), slots)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        append_kv(x, x, cache, torch.zeros(6, 2, 64, device=dev, dtype=BF16, requires_grad=True), slots)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        gather_kv(cache, torch.zeros(6, 2, 64, device=dev, dtype=BF16, requires_grad=True), slots, BF16)
+    assert not cache.any()
+    version = cache._version
+    append_kv(x, x, cache, cache.clone(), slots)
+    assert cache._version == version + 1

@@ -74,9 +74,9 @@ def test_types(dev, axes, table_dtype, index_dtype, weight_dtype):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("axes", ["one", "blocks", "alternating"])
 def test_many_heads_per_lane_group(dev, axes, interleaved):
-    """Launches that fill the chip take four heads of a token at a time; head counts that are no multiple of four."""
-    for hq, hk in ((61, 7), (64, 2)):
-        run(4100, hq, hk, 128, 128, interleaved, axes, BF16, F32, torch.int64, BF16)
+    """Launches that fill the chip may take two or four heads of a token at a time; head counts that are no multiple of either."""
+    for hq, hk, dim, width in ((61, 7, 128, 128), (64, 2, 128, 64), (61, 7, 72, 72), (64, 2, 80, 40)):
+        run(1030, hq, hk, dim, width, interleaved, axes, BF16, F32, torch.int64, BF16)
 
 
 def test_section_counts(dev):
@@ -201,3 +201,47 @@ def test_other_stream_and_graph(dev):
         want = norm_rotate_qk(q, k, w, w, EPS, positions, cos_sin)
         assert torch.equal(q_out, want[0]) and torch.equal(k_out, want[1])
         del other
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("axes", [1, 3])
+@pytest.mark.parametrize("dim", [128, 72, 90])
+def test_a_token_alone_and_among_others(dev, dim, axes, dtype):
+    """The same bits whatever else is in the batch."""
+    g = torch.Generator().manual_seed(13)
+    q, k = heads(g, 1100, 61, dim, dtype=dtype).to(dev), heads(g, 1100, 7, dim, dtype=dtype).to(dev)
+    w = (torch.rand(dim, generator=g) + 0.5).to(dev)
+    cos_sin = table(300, dim).to(dev)
+    third = dim // 6
+    turn = dict(sections=[dim // 2 - 2 * third, third, third], alternating=True) if axes == 3 else {}
+    positions = torch.randint(0, 300, (axes, 1100) if axes == 3 else (1100,), generator=g).to(dev)
+    for norm in (False, True):
+        call = (lambda q, k, p: norm_rotate_qk(q, k, w, w, EPS, p, cos_sin, **turn)) if norm else (lambda q, k, p: rotate_qk(q, k, p, cos_sin, **turn))
+        whole = call(q, k, positions)
+        for at in (0, 517, 1099):
+            one = call(q[at:at + 1], k[at:at + 1], positions[..., at:at + 1])
+            assert torch.equal(one[0], whole[0][at:at + 1]) and torch.equal(one[1], whole[1][at:at + 1])
+
+
+def test_gradients_and_tracers_are_refused(dev):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    cos_sin, positions = table(10, 64).to(dev), torch.arange(3, device=dev)
+    x = torch.ones(3, 2, 64, device=dev, dtype=BF16)
+    leaf = torch.ones(3, 2, 64, device=dev, dtype=BF16, requires_grad=True)
+    w = torch.ones(64, device=dev, requires_grad=True)
+    for call in (lambda: rotate_qk(leaf, x, positions, cos_sin), lambda: rotate_qk(x, leaf, positions, cos_sin),
+                 lambda: norm_rotate_qk(x, x, w, w, EPS, positions, cos_sin)):
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with pytest.raises(NotImplementedError):
+        torch.vmap(lambda q: rotate_qk(q, None, positions, cos_sin)[0])(torch.ones(4, 3, 2, 64, device=dev, dtype=BF16))
+    with FakeTensorMode() as mode:
+        with pytest.raises(NotImplementedError):
+            rotate_qk(mode.from_tensor(x), None, mode.from_tensor(positions), mode.from_tensor(cos_sin))
+    out = torch.empty_like(x)
+    version = out._version
+    rotate_qk(x, None, positions, cos_sin, q_out=out)
+    assert out._version == version + 1
