@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256, V == 8 && HEADS == 1 ? 8 : 1) void head_rows_k
       }
     }
   }
-  typename Piece<V>::type raw_w0[K], raw_w1[K];
+  typename Piece<V>::type raw_w0[K] = {}, raw_w1[K] = {};
   if (NORM && p.w && !p.w_is_f32) {
 #pragma unroll
     for (int j = 0; j < K; j++) {

@@ -537,7 +537,7 @@ extern "C" int sglamd_ue8m0_linear_operands(const void* input, int in_dtype, voi
 }
 
 extern "C" const char* sglamd_last_error(void) { return g_err; }
-extern "C" int sglamd_abi_version(void) { return 8; }
+extern "C" int sglamd_abi_version(void) { return 9; }
 
 extern "C" int sglamd_per_token_group_quant_8bit(const void* input, int in_dtype, void* output_q, int q_dtype,
                                                  void* output_s, int64_t rows, int64_t hidden, int group_size,
