@@ -64,7 +64,7 @@ def check_8(codes, want, off, given=None, scales=None, group=None):
     """8-bit codes of rows whose 64-bit values are `want` [..., dim]: with a given scale (broadcastable to want), or with the scales
     that came back [..., dim / group]."""
     group = group or want.shape[-1]
-    grouped = lambda t: t.reshape(*t.shape[:-1], -1, group)  # noqa: E731
+    grouped = lambda t: t.reshape(*t.shape[:-1], t.shape[-1] // group, group)  # noqa: E731
     int8 = codes.dtype == torch.int8
     value = codes.cpu().double() if int8 else codes.cpu().float().double()
     if given is None:
