@@ -507,13 +507,15 @@ Tensor int8_weight_sums(const Tensor& weight) {
 // The memory of a tensor, for calls that write into tensors they are given.
 struct Span {
   const uint8_t *begin, *end;  // all of it lies in [begin, end)
-  int64_t item, dims = 0, sizes[4], strides[4];  // bytes; dimensions of more than one element
-  explicit Span(const Tensor& t) : begin((const uint8_t*)t.data_ptr()), end(begin), item(t.element_size()) {
+  int64_t item, dims, sizes[4], strides[4];  // bytes; dimensions of more than one element
+  void of(const Tensor& t) {
+    begin = end = (const uint8_t*)t.data_ptr(), item = (int64_t)t.element_size(), dims = 0;
     if (t.numel() == 0) return;
     end += item;
-    for (int64_t d = 0; d < t.dim(); d++)
-      if (t.size(d) > 1) {
-        sizes[dims] = t.size(d), strides[dims] = t.stride(d) * item;
+    const at::IntArrayRef all_sizes = t.sizes(), all_strides = t.strides();
+    for (size_t d = 0; d < all_sizes.size(); d++)
+      if (all_sizes[d] > 1) {
+        sizes[dims] = all_sizes[d], strides[dims] = all_strides[d] * item;
         end += (sizes[dims] - 1) * strides[dims];
         dims++;
       }
@@ -566,7 +568,7 @@ void* address(const Tensor& t) {
 // One call: its tensors, what it writes, and the structures of the C interface.
 struct HeadsCall {
   const char* op;
-  sglamd_heads part[4] = {};
+  sglamd_heads part[3] = {};
   sglamd_gather back[2] = {};
   int parts = 0;
   sglamd_rotation rotation = {};
@@ -577,7 +579,7 @@ struct HeadsCall {
     const char* name;
     int from;  // written: the read operand that it may be one and the same tensor with, or -1
   };
-  Operand reads[16], writes[8];  // (the longest call has 13 and 6)
+  Operand reads[16], writes[8];  // (the longest call has 10 and 6)
   int num_reads = 0, num_writes = 0;
 
   explicit HeadsCall(const char* name) : op(name) {}
@@ -743,13 +745,15 @@ struct HeadsCall {
     if (observed)
       C10_THROW_ERROR(NotImplementedError, std::string(op) + " has no gradient and takes plain tensors only, outside of tracers and "
                                                              "transforms (call it under torch.no_grad())");
-    for (int i = 0; i < num_writes; i++) {
-      const Span to(*writes[i].tensor);
-      TORCH_CHECK(is_apart(to), writes[i].name, " must not be expanded or overlap itself");
-      for (int j = 0; j < i; j++) TORCH_CHECK(disjoint(to, Span(*writes[j].tensor)), writes[i].name, " must not overlap ", writes[j].name);
-      for (int j = 0; j < num_reads; j++) {
-        const Span from(*reads[j].tensor);
-        TORCH_CHECK((writes[i].from == j && to.same(from)) || disjoint(to, from), writes[i].name, " must not overlap ", reads[j].name);
+    if (num_writes) {
+      Span from[16], to[8];
+      for (int j = 0; j < num_reads; j++) from[j].of(*reads[j].tensor);
+      for (int i = 0; i < num_writes; i++) {
+        to[i].of(*writes[i].tensor);
+        TORCH_CHECK(is_apart(to[i]), writes[i].name, " must not be expanded or overlap itself");
+        for (int j = 0; j < i; j++) TORCH_CHECK(disjoint(to[i], to[j]), writes[i].name, " must not overlap ", writes[j].name);
+        for (int j = 0; j < num_reads; j++)
+          TORCH_CHECK((writes[i].from == j && to[i].same(from[j])) || disjoint(to[i], from[j]), writes[i].name, " must not overlap ", reads[j].name);
       }
     }
     for (int i = 0; i < num_reads + num_writes; i++) {

@@ -426,3 +426,30 @@ def test_gradients_are_refused(dev):
     version = cache._version
     append_kv(x, x, cache, cache.clone(), slots)
     assert cache._version == version + 1
+
+
+def test_behind_a_quantised_projection(dev):
+    """A layer's input as this library runs it: residual, norm and int8 codes, the int8 qkv product, heads into an int8 cache, the
+    context back.  The heads' values are the product's own output, rounded to int8 rows once."""
+    from sglang_amd.quantization.fused_row_quant import fused_rms_row_quant
+    from sglang_amd.quantization.int8_utils import apply_int8_linear, int8_weight_sums
+
+    g = torch.Generator().manual_seed(16)
+    tokens, hidden, hq, hk, dim = 21, 1024, 8, 2, 128
+    x, res = (torch.randn(tokens, hidden, generator=g).to(BF16).cuda() for _ in range(2))
+    gamma = (torch.rand(hidden, generator=g) + 0.5).to(BF16).cuda()
+    w = torch.randint(-127, 128, ((hq + 2 * hk) * dim, hidden), generator=g).to(torch.int8).cuda()
+    wscale = (torch.rand(w.shape[0], 1, generator=g) * 1e-4 + 1e-4).cuda()
+    (q8, s8, zp), _, _ = fused_rms_row_quant(x, gamma, EPS, res=res, symmetric=False)
+    qkv = apply_int8_linear(q8, w.t(), wscale, weight_sums=int8_weight_sums(w.t()), input_scale=s8, input_zero_point=zp, out_dtype=BF16)
+    qkv = qkv.view(tokens, hq + 2 * hk, dim)
+    (kc, ks), (vc, vs) = (make_cache(g, "int8_rows", 4, 16, (hk, dim), BF16) for _ in range(2))
+    slots, positions, cos_sin = torch.randperm(64, generator=g)[:tokens].cuda(), torch.arange(tokens, device=dev), table(64, dim).cuda()
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    q_out, _ = append_kv(k, v, kc, vc, slots, k_scale=ks, v_scale=vs, q=q, positions=positions, cos_sin=cos_sin)
+    check_16(q_out, *turned(*normed(q, None, EPS), positions, cos_sin, False))
+    want = turned(*normed(k, None, EPS), positions, cos_sin, False)[0], v.cpu().double()
+    for got, rows in zip(gather_kv(kc, vc, slots, BF16, k_scale=ks, v_scale=vs), want):
+        step = rows.abs().amax(dim=-1, keepdim=True) / 127
+        # half a step of int8, half a step of bfloat16; 2^-20 for the scale and the rotation
+        assert ((got.cpu().double() - rows).abs() <= (step * 0.5 * (1 + 2.0 ** -8) + rows.abs() * 2.0 ** -8) * (1 + 2.0 ** -20) + step * 2.0 ** -13).all()
