@@ -632,8 +632,8 @@ typedef struct {
 } sglamd_slots;
 
 /* Rotary positions.  The table has a row of width / 2 cosines and then width / 2 sines per position, table_dtype F32 or the heads'
- * type, rows table_stride elements apart.  Pair i < width / 2 of a head is (x[i], x[i + width / 2]), interleaved: (x[2 i], x[2 i + 1]);
- * (a, b) becomes (a cos - b sin, b cos + a sin), the values behind the first `width` stay.  The position of token t on axis k is
+ * type, rows table_stride elements apart, one position at least and 2 GiB at most.  Pair i < width / 2 of a head is
+ * (x[i], x[i + width / 2]), interleaved: (x[2 i], x[2 i + 1]);  (a, b) becomes (a cos - b sin, b cos + a sin), the values behind the first `width` stay.  The position of token t on axis k is
  * positions[k * axis_stride + t * position_stride], I32 or I64.  With more than one axis, sections[k] pairs turn by axis k: the
  * first sections[0] by axis 0 and so on, alternating: pair i by axis i % axes where i < axes * sections[i % axes], by axis 0
  * otherwise.  A position outside of the table gives NaN. */

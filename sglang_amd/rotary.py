@@ -1,8 +1,8 @@
 """Rotary positions on the heads of queries and keys, with RMSNorm of every head in front of it where a model has one.
 
 Heads are half/bfloat16 [tokens, heads, head size] with contiguous rows (views into a projection's output will do; head size even, at
-most 1024).  cos_sin [positions, R], float32 or of the heads' dtype, holds R / 2 cosines and then R / 2 sines per position, R at
-most the head size.  Pair i < R / 2 of a head is (x[i], x[i + R / 2]), with `interleaved` (x[2 i], x[2 i + 1]); (a, b) becomes
+most 1024).  cos_sin [positions, R], float32 or of the heads' dtype, at most 2 GiB, holds R / 2 cosines and then R / 2 sines per position, R
+even and at most the head size.  Pair i < R / 2 of a head is (x[i], x[i + R / 2]), with `interleaved` (x[2 i], x[2 i + 1]); (a, b) becomes
 (a cos - b sin, b cos + a sin) and the values behind the first R stay.
 
 positions (int32 or int64) is [tokens], or [axes, tokens] with `sections`, how many pairs turn by each of up to four axes (the time,

@@ -255,6 +255,9 @@ def test_c_interface_refuses_before_any_launch():
             (b"even, 2 to 1024", 1, 2, heads(rotate=1), rotation(width=0), None),
             (b"a rotated width of 128 in heads of 64", 1, 2, heads(rotate=1), rotation(width=128), None),
             (b"a table of 0 positions", 1, 2, heads(rotate=1), rotation(table_rows=0), None),
+            (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_rows=(1 << 23) + 1), None),
+            (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_dtype=2, table_rows=(1 << 24) + 1), None),
+            (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_stride=1 << 40), None),
             (b"null table", 1, 2, heads(rotate=1), rotation(positions=None), None),
             (b"positions must be", 1, 2, heads(rotate=1), rotation(positions_dtype=0), None),
             (b"the table must be", 1, 2, heads(rotate=1), rotation(table_dtype=1), None),
