@@ -681,11 +681,12 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
     SGLAMD_REQUIRE(r.positions_dtype == SGLAMD_I32 || r.positions_dtype == SGLAMD_I64, SGLAMD_EINVAL, "%s: positions must be I32 or I64", op);
     SGLAMD_REQUIRE(r.width > 0 && r.width % 2 == 0 && r.width <= 1024, SGLAMD_EINVAL, "%s: a rotated width of %lld: even, 2 to 1024", op,
                    (long long)r.width);
-    SGLAMD_REQUIRE(r.table_rows > 0 && r.table_rows < (1ll << 31) && r.table_stride >= 0 &&
-                       (r.table_rows - 1) * r.table_stride + r.width <= (1ll << (r.table_dtype == SGLAMD_F32 ? 29 : 30)),
+    const int64_t stride = r.table_rows > 1 ? r.table_stride : 0;
+    SGLAMD_REQUIRE(r.table_rows > 0 && r.table_rows < (1ll << 31) && stride >= 0 && stride < (1ll << 31) &&
+                       (r.table_rows - 1) * stride + r.width <= (1ll << (r.table_dtype == SGLAMD_F32 ? 29 : 30)),
                    SGLAMD_EINVAL, "%s: a table of %lld positions: one to 2 GiB are served", op, (long long)r.table_rows);
     SGLAMD_REQUIRE(r.axes >= 1 && r.axes <= 4, SGLAMD_EINVAL, "%s: one to four position axes", op);
-    a.table = r.cos_sin, a.table_stride = r.table_stride, a.table_rows = r.table_rows, a.table_is_f32 = r.table_dtype == SGLAMD_F32;
+    a.table = r.cos_sin, a.table_stride = stride, a.table_rows = r.table_rows, a.table_is_f32 = r.table_dtype == SGLAMD_F32;
     a.positions = r.positions, a.positions_are_i64 = r.positions_dtype == SGLAMD_I64;
     a.axis_stride = r.axis_stride, a.position_stride = r.position_stride;
     a.pairs = (int)(r.width / 2), a.axes = r.axes;

@@ -258,6 +258,8 @@ def test_c_interface_refuses_before_any_launch():
             (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_rows=(1 << 23) + 1), None),
             (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_dtype=2, table_rows=(1 << 24) + 1), None),
             (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_stride=1 << 40), None),
+            (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_rows=(1 << 31) - 1, table_stride=1 << 62), None),
+            (b"one to 2 GiB", 1, 2, heads(rotate=1), rotation(table_stride=-64), None),
             (b"null table", 1, 2, heads(rotate=1), rotation(positions=None), None),
             (b"positions must be", 1, 2, heads(rotate=1), rotation(positions_dtype=0), None),
             (b"the table must be", 1, 2, heads(rotate=1), rotation(table_dtype=1), None),
