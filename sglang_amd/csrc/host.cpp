@@ -534,7 +534,48 @@ struct Span {
   }
 };
 
-// Whether two spans share no byte: apart, or side by side within every step of a stride of theirs (views of one row).
+// How far apart an element of one span and one of another lie: multiples of the strides of both, forward in the one and back in
+// the other.  Strides that both have come together, the largest first.
+struct Distances {
+  struct Step {
+    int64_t stride, least, most;
+  };
+  Step steps[8];
+  int64_t low[9], high[9];  // what the steps from i on reach
+  int n = 0, tries = 4096;
+
+  void add(int64_t stride, int64_t least, int64_t most) {
+    if (stride == 0) return;
+    int i = n;
+    while (i > 0 && steps[i - 1].stride < stride) i--;
+    if (i > 0 && steps[i - 1].stride == stride) {
+      steps[i - 1].least += least, steps[i - 1].most += most;
+      return;
+    }
+    for (int j = n++; j > i; j--) steps[j] = steps[j - 1];
+    steps[i] = {stride, least, most};
+  }
+  Distances(const Span& a, const Span& b) {
+    for (int64_t d = 0; d < a.dims; d++) add(a.strides[d], 0, a.sizes[d] - 1);
+    for (int64_t d = 0; d < b.dims; d++) add(b.strides[d], 1 - b.sizes[d], 0);
+    low[n] = high[n] = 0;
+    for (int i = n - 1; i >= 0; i--) low[i] = low[i + 1] + steps[i].least * steps[i].stride, high[i] = high[i + 1] + steps[i].most * steps[i].stride;
+  }
+  // Whether the steps from i on come to a number in [from, to].  Only multiples whose rest the smaller steps can make up for are gone
+  // into: one or two of a stride in layouts that are nested alike.  After many tries, of others, the answer is that they may.
+  bool reach(int i, int64_t from, int64_t to) {
+    if (i == n) return from <= 0 && 0 <= to;
+    const Step& s = steps[i];
+    const auto down = [&](int64_t x) { return x >= 0 ? x / s.stride : -((s.stride - 1 - x) / s.stride); };
+    const int64_t first = std::max(s.least, -down(high[i + 1] - from)), last = std::min(s.most, down(to - low[i + 1]));
+    for (int64_t k = first; k <= last; k++)
+      if (--tries < 0 || reach(i + 1, from - k * s.stride, to - k * s.stride)) return true;
+    return false;
+  }
+};
+
+// Whether two spans share no byte: apart, side by side within every step of a stride of theirs (views of one row; most calls end
+// here), or with no two elements closer than their sizes (pages with something else behind their slots).
 bool disjoint(const Span& a, const Span& b) {
   if (a.begin == a.end || b.begin == b.end || a.end <= b.begin || b.end <= a.begin) return true;
   for (const Span* of : {&a, &b})
@@ -545,7 +586,8 @@ bool disjoint(const Span& a, const Span& b) {
       const int64_t at = ((b.begin - a.begin) % step + step) % step;
       if (ra >= 0 && rb >= 0 && ra <= at && at + rb <= step) return true;
     }
-  return false;
+  const int64_t between = b.begin - a.begin;
+  return !Distances(a, b).reach(0, between - a.item + 1, between + b.item - 1);
 }
 
 // Whether no element of a tensor shares its place with another one.
