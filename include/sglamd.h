@@ -624,7 +624,8 @@ int sglamd_fp8_blockwise_scaled_grouped_mm(void* output, int out_dtype, const vo
 /* A cache of `pages` pages of `page_size` slots and the slot of every token (a gathered row: the slot that it comes from), I32 or
  * I64, slot_stride elements apart.  Slot s is row s % page_size of page s / page_size.  A slot outside [0, pages * page_size) is
  * none: such a token writes nothing to the cache, such a gathered row is zeros.  Slots of one launch that write have to differ:
- * where two are the same, each 2 to 32 bytes of the row are of one of the two tokens.  pages * page_size < 2^31. */
+ * where two are the same, each value of the row is of one of the two tokens, and so is its scale, not always of the same one.
+ * pages * page_size < 2^31. */
 typedef struct {
   const void* slots;
   int slots_dtype;
@@ -633,10 +634,10 @@ typedef struct {
 
 /* Rotary positions.  The table has a row of width / 2 cosines and then width / 2 sines per position, table_dtype F32 or the heads'
  * type, rows table_stride elements apart, one position at least and 2 GiB at most.  Pair i < width / 2 of a head is
- * (x[i], x[i + width / 2]), interleaved: (x[2 i], x[2 i + 1]);  (a, b) becomes (a cos - b sin, b cos + a sin), the values behind the first `width` stay.  The position of token t on axis k is
- * positions[k * axis_stride + t * position_stride], I32 or I64.  With more than one axis, sections[k] pairs turn by axis k: the
- * first sections[0] by axis 0 and so on, alternating: pair i by axis i % axes where i < axes * sections[i % axes], by axis 0
- * otherwise.  A position outside of the table gives NaN. */
+ * (x[i], x[i + width / 2]), interleaved: (x[2 i], x[2 i + 1]);  (a, b) becomes (a cos - b sin, b cos + a sin), the values behind
+ * the first `width` stay.  The position of token t on axis k is positions[k * axis_stride + t * position_stride], I32 or I64.  With
+ * more than one axis, sections[k] pairs turn by axis k: the first sections[0] by axis 0 and so on, alternating: pair i by axis
+ * i % axes where i < axes * sections[i % axes], by axis 0 otherwise.  A position outside of the table gives NaN. */
 typedef struct {
   const void* cos_sin;
   int table_dtype;
@@ -652,12 +653,15 @@ typedef struct {
 
 /* One tensor x of heads [tokens, heads, dim], strides in elements, dim contiguous, even, at most 1024.  In fp32, rounded once at
  * the end:  y = x;  with a weight (F32 or the heads' type, [dim]) y = x / sqrt(mean(x^2) + eps) * weight over each head (a head
- * whose sum of squares is not finite in fp32 is NaN);  rotate: its first rotation.width values turned.
+ * whose sum of squares is not finite in fp32 is NaN; with an eps of zero, values below 1e-19, whose squares are below fp32's normal
+ * range, lose digits);  rotate: its first rotation.width values turned.
  *   out    optional: y in the heads' type; may be x itself
  *   cache  optional: y in the slots' rows, strides in elements; cache_dtype the heads' type, or
- *          FP8_E4M3: code = e4m3(clamp(y / scale, -448, 448)) with given_scale[head * given_head], or with
- *                    scale = max|y| / 448 of each row, written to `scales`
- *          I8:       code = round(y / scale), scale = max(max|y|, 1e-10) / 127 of each row, written to `scales`
+ *          FP8_E4M3: code = e4m3(clamp(y * (1 / scale), -448, 448)) with given_scale[head * given_head], or with
+ *                    scale = max|y| / 448 of each row, written to `scales`; zeros for a scale of zero
+ *          I8:       with m = max(max|y|, 1e-10) of each row: scale = m / 127, written to `scales`, code = round(y * (127 / m)),
+ *                    halves away from zero
+ *          (1 / scale and 127 / m in fp32, as the row quantisers have it: next to a tie a code may be the other one of the two)
  *          scale_group: dim (one scale per row), or 128: one per 128 values, scales_group elements apart, for heads that are
  *          not rotated and whose dim is a multiple of 128.  A row that holds a NaN or an infinity gets such a scale.
  * Memory that is written overlaps nothing else that the launch reads or writes, but for out == x. */

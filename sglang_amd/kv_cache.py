@@ -4,16 +4,19 @@ rows of a context back in 16 bits.
 A cache is [slots, heads, head size], or [pages, page size, heads, head size] in any order of memory with contiguous rows (a cache
 that keeps the heads of a page together is passed transposed).  Slot s is row s % page size of page s / page size.  `slots` (int32
 or int64, one per token) outside of the cache stand for no slot: padding, whose rows are not written, or read as zeros.  Slots that
-are written in one call have to differ (of two tokens with the same slot, either may be kept, or parts of both).
+are written in one call have to differ (of two tokens with the same slot, either may be kept, or parts of both, its codes with the
+other one's scale among them).
 
 A cache of the heads' dtype has no scale.  An 8-bit one holds, with y the row in float32:
 
-  float8_e4m3fn, scale float32 [1], or [heads]     code = e4m3(clamp(y / scale, -448, 448)), the scale known beforehand
+  float8_e4m3fn, scale float32 [1], or [heads]     code = e4m3(clamp(y * (1 / scale), -448, 448)), the scale known beforehand
   float8_e4m3fn, scale float32 [slots..., heads]   scale = max|y| / 448 of the token's head, written to the slot's place
-  int8, scale float32 [slots..., heads]            scale = max(max|y|, 1e-10) / 127, code = round(y / scale)
+  int8, scale float32 [slots..., heads]            m = max(max|y|, 1e-10), scale = m / 127, code = round(y * (127 / m))
 
-where [slots...] are the cache's own leading dimensions; a row that holds a NaN or an infinity gets a scale that is one.  Rows
-beyond those of `slots` are left as they are, and their scales too.
+where [slots...] are the cache's own leading dimensions; a row that holds a NaN or an infinity gets a scale that is one.  1 / scale
+and 127 / m are rounded to float32, as in the row quantisers: next to a tie a code may be the other one of the two.  A scale of
+zero gives codes of zero; int8 rounds halves away from zero.  Rows beyond those of `slots` are left as they are, and their
+scales too.
 
 Memory that is written overlaps nothing else that a call is given.  There is no gradient and no torch.ops schema: under a tracer or a
 transform the functions raise NotImplementedError."""

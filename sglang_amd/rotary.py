@@ -50,5 +50,6 @@ def norm_rotate_qk(
     k_out: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """rotate_qk of the normalised heads x / sqrt(mean(x^2) + epsilon) * weight, the weights [head size] float32 or of the heads'
-    dtype.  A head whose sum of squares is not finite in float32 is NaN."""
+    dtype.  A head whose sum of squares is not finite in float32 is NaN; with an epsilon of zero, values below 1e-19, whose squares are
+    below float32's normal range, lose digits."""
     return _C.norm_rotate_qk(q, k, q_weight, k_weight, epsilon, positions, cos_sin, interleaved, sections, alternating, q_out, k_out)
