@@ -9,10 +9,11 @@
 //
 // All of it is bound by HBM at prompt sizes (some ten operations per value, each value read once and written once) and by the launch
 // at decode sizes, so one launch does everything that a layer needs between its projection and its attention.  Measured
-// against a copy of as many bytes (5.05 TB/s): 8191 tokens of 64 + 2 x 8 heads of 128, rotated, into e4m3 rows 5.2 TB/s; 4096 tokens
-// of 128 rotary parts, 128 bytes in each 384, 4.4 (a copy of such pieces 4.5); gathered int8 rows 5.0; heads with a norm 4.3 to 4.5.
+// against a copy of as many bytes (5.05 TB/s): 8191 tokens of 64 + 2 x 8 heads of 128, rotated, into e4m3 rows 5.4 TB/s; 4096 tokens
+// of 128 rotary parts, 128 bytes in each 384, 4.5 (a copy of such pieces 4.6); gathered int8 rows 5.0; heads with a norm 4.5 to 4.7,
+// alternating axes 4.2.  Written are exactly the outputs' bytes, read 1.01 to 1.07 of the inputs' (counters).
 // What decided it, in this order: pieces in words (a piece of eight 16-bit values that may not be there was held in
-// eight registers), one head per lane group in at most 64 registers instead of four in 160 (4.3 to 5.2 TB/s), loads without
+// eight registers), one head per lane group in at most 64 registers (four heads: 4.9 TB/s instead of 5.4), loads without
 // conditions (a condition between two loads makes the first wait for both), and the kernel's arguments touched at the start.
 #include <utility>
 
@@ -732,13 +733,17 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   const int k = v == 1 ? 8 : 1;
 
   // One head per lane group: 57 to 64 registers, eight waves a SIMD, and the most loads in flight (8191 tokens of 64 + 2 x 8 heads
-  // of 128 into e4m3 rows: 62 us, two heads 64, four 67).  With several axes a lane may need sixteen loads for its pairs, which
-  // two heads share once there are enough of them to fill half of the chip (2901 tokens of 32 heads, alternating axes: 13.0 us, one
-  // head 15.8, four 12.2; 4096 of 72, normalised: 38.5, 44.2, 37.4; blocks of axes: 35.8, 37.4, 36.5).
+  // of 128 into e4m3 rows: 59.9 us, two heads 62.3, four 66.1).  With several axes a lane may need sixteen loads for its pairs, which
+  // two heads share from 1024 lanes a CU on, half of what it holds.  One | two | four heads, us in a graph, tokens x heads of 128:
+  //   alternating     256 x 32  4.1 | 4.4 | 5.3    768 x 32  6.8 | 6.3 | 6.2    1024 x 32  8.5 | 7.3 | 7.2    2901 x 32  15.9 | 13.1 | 12.2
+  //   with a norm     256 x 32  4.6 | 5.2 | 6.8    768 x 32  7.4 | 7.3 | 7.7    1024 x 32  9.1 | 8.2 | 8.7    4096 x 72  42.1 | 36.7 | 36.5
+  //   blocks of axes  256 x 32  3.4 | 3.8 | 4.4   1024 x 32  5.6 | 5.8 | 6.2    2901 x 32  10.5 | 10.3 | 10.3   4096 x 72  34.5 | 33.2 | 35.5
+  // Two for both kinds of sections, one rule: four would be 7 to 9 % faster for 2901 tokens of 32 heads and more where axes alternate,
+  // and is no faster for 72 heads; one up to 4 % faster for blocks of axes between 1024 and 2048 tokens of 32.
   int64_t lanes = 0;
   for (int i = 0; i < num_parts; i++) lanes += tokens * parts[i].heads << log2_up(ceil_div(parts[i].dim, 2 * v * k));
-  // Pieces of four: the lanes' addresses are most of the work, four heads share them (4096 tokens of 72 heads of 72, normalised: 28 us,
-  // two heads 31, eight 31, one 39; 500 of 80 heads of 72 into e4m3 rows: four 8.3, one 7.0).
+  // Pieces of four: the lanes' addresses are most of the work, four heads share them (4096 tokens of 72 heads of 72, normalised:
+  // 27.2 us, two heads 30.6, eight 30.7, one 38.7; 500 of 80 heads of 72 into e4m3 rows: four 7.6, two 6.1, one 7.2).
   const DeviceScope scope;
   const int64_t cus = device_cus();
   const int many = v == 4 && lanes >= cus * 4096 ? HEADS_OF_FOURS : v == 8 && a.axes > 1 && lanes >= cus * 1024 ? HEADS_MANY : 1;
@@ -827,8 +832,8 @@ extern "C" int sglamd_gather_head_rows(const sglamd_gather* parts, int num_parts
     while (v > 1 && g.dim % v) v /= 2;
   }
   if (v == 2) v = 1;
-  // Four units a lane once one each fills the chip several times over (int8 rows of 2 x 8 x 128, one | four: 500 of them 2.7 | 4.2 us,
-  // 10000 13.3 | 15.4, 20000 30.8 | 28.6, 65000 92.8 | 80.9).
+  // Four units a lane once one each fills the chip several times over (int8 rows of 2 x 8 x 128, one | four: 500 of them 2.6 | 4.0 us,
+  // 10000 13.5 | 13.7, 20000 30.6 | 28.4, 65000 92.9 | 80.6).
   const DeviceScope scope;
   int64_t all = 0;
   for (int i = 0; i < num_parts; i++) all += rows * parts[i].heads * (parts[i].dim / v);
