@@ -739,7 +739,7 @@ extern "C" int sglamd_head_rows(const sglamd_heads* parts, int num_parts, int64_
   //   with a norm     256 x 32  4.6 | 5.2 | 6.8    768 x 32  7.4 | 7.3 | 7.7    1024 x 32  9.1 | 8.2 | 8.7    4096 x 72  42.1 | 36.7 | 36.5
   //   blocks of axes  256 x 32  3.4 | 3.8 | 4.4   1024 x 32  5.6 | 5.8 | 6.2    2901 x 32  10.5 | 10.3 | 10.3   4096 x 72  34.5 | 33.2 | 35.5
   // Two for both kinds of sections, one rule: four would be 7 to 9 % faster for 2901 tokens of 32 heads and more where axes alternate,
-  // and is no faster for 72 heads; one up to 4 % faster for blocks of axes between 1024 and 2048 tokens of 32.
+  // and is no faster for 72 heads; one up to 5 % faster for blocks of axes at 1024 to 2901 tokens of 32.
   int64_t lanes = 0;
   for (int i = 0; i < num_parts; i++) lanes += tokens * parts[i].heads << log2_up(ceil_div(parts[i].dim, 2 * v * k));
   // Pieces of four: the lanes' addresses are most of the work, four heads share them (4096 tokens of 72 heads of 72, normalised:
